@@ -14,6 +14,8 @@ from .llama import mixtral_8x7b, LlamaArch, QLlamaAttention, QLlamaDecoderLayer,
 from .module import QLinear  # noqa: F401
 from .ops import FP16AccumMatMul, FP32AccumMatMul  # noqa: F401
 from .ptq import PTQConfig, load_quant_config  # noqa: F401
+from .attention import shared_prefix_attention, window_attention  # noqa: F401
+from .rotary import qk_norm_rope, rope_frequencies, rope_rotate  # noqa: F401
 from .ep_moe import ExpertParallelMoE, QuantExpert  # noqa: F401
 from .tp_linear import ColumnParallelQLinear, RowParallelQLinear  # noqa: F401
 from .quantizer import (HBQQuantizer, MXExQuantizer, MXFPQuantizer, MXINTQuantizer, PackedTensor,  # noqa: F401
@@ -23,4 +25,5 @@ from .quantizer import (HBQQuantizer, MXExQuantizer, MXFPQuantizer, MXINTQuantiz
 __all__ = ["HBQQuantizer", "MXFPQuantizer", "MXINTQuantizer", "MXExQuantizer", "VSQQuantizer", "_QBase", "FP16AccumMatMul", "QLinear",
            "PTQConfig", "load_quant_config", "blockquant_ext", "gemm", "gemm_status", "gemm_status_reset", "PackedTensor",
            "dequantize_packed", "HbqError", "launch_count", "get_max_norm", "get_min_norm", "get_min_subnorm",
-           "write_k_cache", "write_v_cache", "swiglu_quantize", "rmsnorm_quantize", "softmax_quantize", "ColumnParallelQLinear", "RowParallelQLinear", "LlamaArch", "mixtral_8x7b", "FP32AccumMatMul", "QLlamaModel", "QLlamaAttention", "QLlamaMLP", "QLlamaDecoderLayer", "ExpertParallelMoE", "QuantExpert", "W4Weight", "gemm_reserve_sms"]
+           "write_k_cache", "write_v_cache", "swiglu_quantize", "rmsnorm_quantize", "softmax_quantize", "ColumnParallelQLinear", "RowParallelQLinear", "LlamaArch", "mixtral_8x7b", "FP32AccumMatMul", "QLlamaModel", "QLlamaAttention", "QLlamaMLP", "QLlamaDecoderLayer", "ExpertParallelMoE", "QuantExpert", "W4Weight", "gemm_reserve_sms",
+           "rope_frequencies", "rope_rotate", "qk_norm_rope", "window_attention", "shared_prefix_attention"]

@@ -28,6 +28,7 @@ EXPORTS = [
     "hbq_gemm_kn_noalloc", "hbq_gemm_w4", "hbq_gemm_w4_prepack", "hbq_gemm_w4_prepacked_bytes",
     "hbq_gemm_w4_workspace_bytes", "hbq_kv_write_k", "hbq_kv_write_v", "hbq_swiglu_quantize", "hbq_rmsnorm_quantize", "hbq_softmax_quantize",
     "hbq_rope_heads", "hbq_quantize_q_runs", "hbq_quantize_head_rows", "hbq_moe_route", "hbq_gemm_grouped", "hbq_moe_combine",
+    "hbq_rope_rotate", "hbq_qk_norm_rope", "hbq_attention_run", "hbq_attention_workspace_bytes",
     "hbq_gemm_status", "hbq_gemm_status_reset", "hbq_gemm_wait_selftest", "hbq_gemm_reserve_sms", "hbq_gemm_tile_columns", "hbq_error_string", "hbq_last_cuda_error",
     "hbq_version", "hbq_launch_count",
 ]
@@ -45,6 +46,28 @@ class PackedOut(ctypes.Structure):
     """``hbq_packed_out``"""
     _fields_ = [(n, ctypes.c_void_p) for n in (
         "codes", "sign", "scale_u8", "scale_h", "l2_packed", "l2_idx", "scheme")]
+
+
+class Heads(ctypes.Structure):
+    """``hbq_heads``"""
+    _fields_ = [("data", ctypes.c_void_p), ("out", ctypes.c_void_p), ("weight", ctypes.c_void_p), ("heads", ctypes.c_int64),
+                ("stride", ctypes.c_int64 * 3), ("out_stride", ctypes.c_int64 * 3)]
+
+
+class Rotary(ctypes.Structure):
+    """``hbq_rotary``"""
+    _fields_ = [("inv_freq", ctypes.c_void_p), ("positions", ctypes.c_void_p), ("pos_stride", ctypes.c_int64 * 2),
+                ("rot", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("positions_64", ctypes.c_int32), ("factor", ctypes.c_float)]
+
+
+class Attention(ctypes.Structure):
+    """``hbq_attention``"""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "out")] + \
+               [(n, ctypes.c_int64) for n in ("B", "L", "H", "Hkv", "S", "D")] + \
+               [(n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride", "out_stride")] + \
+               [(n, ctypes.c_void_p) for n in ("lengths", "starts", "prefix_k", "prefix_v")] + \
+               [("P", ctypes.c_int64), ("pk_stride", ctypes.c_int64 * 2), ("pv_stride", ctypes.c_int64 * 2),
+                ("window", ctypes.c_int64), ("sinks", ctypes.c_int64), ("scale", ctypes.c_float), ("dtype", ctypes.c_int32)]
 
 
 class HbqError(RuntimeError):
@@ -94,6 +117,11 @@ def lib() -> ctypes.CDLL:
     L.hbq_gemm_grouped.argtypes = [vp, i64, vp, ci, ctypes.POINTER(vp), ctypes.POINTER(vp), ctypes.POINTER(ctypes.c_int32),
                                    i64, i64, ci, ci, ci, vp]
     L.hbq_moe_combine.argtypes = [vp, vp, vp, i64, ci, i64, vp, vp]
+    L.hbq_rope_rotate.argtypes = [ctypes.POINTER(Heads), ctypes.POINTER(Rotary), ci, i64, i64, i64, vp]
+    L.hbq_qk_norm_rope.argtypes = [ctypes.POINTER(Heads), ctypes.POINTER(Heads), ctypes.POINTER(Rotary), ci, i64, i64, i64, ctypes.c_float, vp]
+    L.hbq_attention_run.argtypes = [ctypes.POINTER(Attention), vp, i64, vp]
+    L.hbq_attention_workspace_bytes.argtypes = [ctypes.POINTER(Attention)]
+    L.hbq_attention_workspace_bytes.restype = i64
     L.hbq_gemm_status.argtypes = [ctypes.POINTER(ci)]
     L.hbq_gemm_wait_selftest.argtypes = [vp, vp, vp, i64, i64, i64, ci, ci, ci, ctypes.c_uint32, vp]
     L.hbq_gemm_reserve_sms.argtypes = [ci]
@@ -116,7 +144,7 @@ class _NoHost:
     def quantize(*args):
         return None
 
-    gemm = gemm_w4 = quantize
+    gemm = gemm_w4 = rope_rotate = qk_norm_rope = attention = quantize
 
     @staticmethod
     def current_stream(index):
@@ -141,7 +169,8 @@ def host():
     m = importlib.util.module_from_spec(importlib.util.spec_from_loader("hbq_host", loader))
     loader.exec_module(m)
     m.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (L.hbq_quantize, L.hbq_gemm, L.hbq_gemm_workspace_bytes,
-                                                             L.hbq_gemm_w4)))
+                                                             L.hbq_gemm_w4, L.hbq_rope_rotate, L.hbq_qk_norm_rope,
+                                                             L.hbq_attention_run, L.hbq_attention_workspace_bytes)))
     _host = m
     return m
 

@@ -91,6 +91,9 @@ int gemm_tc_grouped_launch(const void*, int64_t, const int*, int, const void* co
 int moe_route_launch(const int64_t*, int64_t, int, int, int*, int64_t*, int*, cudaStream_t);                      // moe.cu
 int moe_combine_launch(const void*, const void*, const int*, int64_t, int, int64_t, void*, cudaStream_t);
 int rope_heads_launch(const void*, int64_t, int64_t, int64_t, int64_t, const void*, const void*, int64_t, void*, cudaStream_t);   // rope.cu
+int rotary_launch(const hbq_heads*, const hbq_heads*, const hbq_rotary*, int, int64_t, int64_t, int64_t, bool, float, cudaStream_t);   // rotary.cu
+int64_t attention_workspace_bytes(const hbq_attention*);                                                          // attention.cu
+int attention_run(const hbq_attention*, void*, int64_t, cudaStream_t);
 int64_t gemm_w4_prepacked_bytes(int64_t, int64_t, int);
 int gemm_w4_prepack(const hbq_packed_out*, int64_t, int64_t, const hbq_format*, int, void*, cudaStream_t);
 int64_t gemm_w4_workspace_bytes(int64_t, int64_t, int64_t);
@@ -346,6 +349,24 @@ int hbq_gemm_w4(const void* X, const void* Wp, void* C, int64_t M, int64_t N, in
     if (need < 0) return HBQ_ERR_UNSUPPORTED;
     if (!workspace || workspace_bytes < need) return HBQ_ERR_WORKSPACE;
     return gemm_w4_launch(X, Wp, C, M, N, K, fmt, container_bits, bias, workspace, (cudaStream_t)stream, 0);
+}
+
+int hbq_rope_rotate(const hbq_heads* x, const hbq_rotary* r, int dtype, int64_t B, int64_t T, int64_t D, void* stream)
+{
+    return rotary_launch(x, nullptr, r, dtype, B, T, D, false, 0.f, (cudaStream_t)stream);
+}
+
+int hbq_qk_norm_rope(const hbq_heads* q, const hbq_heads* k, const hbq_rotary* r, int dtype, int64_t B, int64_t T, int64_t D,
+                     float eps, void* stream)
+{
+    return rotary_launch(q, k, r, dtype, B, T, D, true, eps, (cudaStream_t)stream);
+}
+
+int64_t hbq_attention_workspace_bytes(const hbq_attention* a) { return attention_workspace_bytes(a); }
+
+int hbq_attention_run(const hbq_attention* a, void* workspace, int64_t workspace_bytes, void* stream)
+{
+    return attention_run(a, workspace, workspace_bytes, (cudaStream_t)stream);
 }
 
 int hbq_gemm_status(int* status_host)

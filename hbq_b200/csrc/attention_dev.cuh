@@ -1,0 +1,47 @@
+// What the attention kernels share: which keys a row sees, and the form in which parts of a row's sum are joined.
+#pragma once
+#include "common.cuh"
+
+namespace hbq {
+
+struct AttnArgs {
+    const void *q, *k, *v, *pk, *pv;
+    void* out;
+    const int32_t *lengths, *starts;
+    int64_t qs[3], ks[3], vs[3], os[3], pks[2], pvs[2];      // strides in elements
+    int64_t S, P, window, sinks;
+    uint32_t B, L, H, Hkv, G, D;
+    float scale_log2;                                        // scale * log2(e)
+    int nsplit;
+    float* part;                                             // [rows][parts][D] sums, then [rows][parts] (maximum, weight)
+    int parts, part0;
+};
+
+// Rows of sequence b: its keys, and the position of its first row.
+__device__ __forceinline__ void sequence_of(const AttnArgs& a, uint32_t b, int64_t* n, int64_t* first)
+{
+    int64_t len = a.lengths ? (int64_t)a.lengths[b] : a.S;
+    len = len < 0 ? 0 : len > a.S ? a.S : len;
+    *n = len;
+    *first = a.starts ? (int64_t)a.starts[b] : len - (int64_t)a.L;
+}
+
+__device__ __forceinline__ float exp2_fast(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// A part's sums and (maximum, weight) of a row; rows are numbered (b * L + i) * H + h.
+__device__ __forceinline__ float* part_sum(const AttnArgs& a, int64_t row, int part) { return a.part + (row * a.parts + part) * a.D; }
+__device__ __forceinline__ float2* part_weight(const AttnArgs& a, int64_t row, int part)
+{
+    return reinterpret_cast<float2*>(a.part + (int64_t)a.B * a.L * a.H * a.parts * a.D) + row * a.parts + part;
+}
+
+int attention_join_launch(const AttnArgs& a, int dtype, cudaStream_t stream);                    // attention_rows.cu
+int attention_rows_launch(AttnArgs& a, int dtype, cudaStream_t stream);
+int64_t attention_rows_parts(const hbq_attention* p, int* nsplit);
+
+}  // namespace hbq

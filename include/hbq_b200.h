@@ -325,6 +325,67 @@ int hbq_gemm_reserve_sms(int n);
  * result on `sms` SMs; sms <= 0: those of the current device that hbq_gemm_reserve_sms leaves. */
 int hbq_gemm_tile_columns(int64_t M, int64_t N, int mode, int sms);
 
+/* ---- rotary positions and head norms ------------------------------------------------------- */
+
+/* A tensor of heads [B, T, heads, D] (fp16 or bf16, values of a head side by side) and where its result goes.
+ * stride: elements from one sequence, token and head to the next, of `data` and of `out`; `out` may be `data` with the
+ * same strides, and else overlaps nothing that is read.  weight: [D], same type (norm only). */
+typedef struct hbq_heads {
+    const void* data;
+    void* out;
+    const void* weight;
+    int64_t heads;
+    int64_t stride[3];
+    int64_t out_stride[3];
+} hbq_heads;
+
+/* The rotation: pair i of a head turns by positions[b, t] * inv_freq[i].  inv_freq: [rot / 2] fp64 on the device; rot
+ * (even, 2 .. D): the values of a head that turn, the first ones.  interleaved: pairs (2 i, 2 i + 1), else
+ * (i, i + rot / 2).  factor: multiplies cosine and sine.  positions: int32 or int64 (positions_64), stride pos_stride. */
+typedef struct hbq_rotary {
+    const double* inv_freq;
+    const void* positions;
+    int64_t pos_stride[2];
+    int32_t rot;
+    int32_t interleaved;
+    int32_t positions_64;
+    float factor;
+} hbq_rotary;
+
+/* Rotary positions with 64-bit angles (apply_rotary_pos_emb, src/module.py:157, for every layout and scaling).
+ * hbq_qk_norm_rope: first each head h becomes h * rsqrt(mean(h^2) + eps) * weight; q and k in one launch (k->heads may
+ * be 0).  32-bit arithmetic, one rounding at the end. */
+int hbq_rope_rotate(const hbq_heads* x, const hbq_rotary* r, int dtype, int64_t B, int64_t T, int64_t D, void* stream);
+int hbq_qk_norm_rope(const hbq_heads* q, const hbq_heads* k, const hbq_rotary* r, int dtype, int64_t B, int64_t T,
+                     int64_t D, float eps, void* stream);
+
+/* ---- attention over a cache ---------------------------------------------------------------- */
+
+/* o = softmax(scale * q k^T) v for rows that see a part of their sequence's keys (fp16 or bf16, fp32 statistics).
+ *   q, out [B, L, H, D], k, v [B, Hkv, S, D], head h reads key head h / (H / Hkv); strides in elements, the last axis
+ *   dense.  Row i of sequence b stands at position p = starts[b] + i (starts NULL: lengths[b] - L + i) and sees key j if
+ *   j < lengths[b] (NULL: S; values are held inside [0, S]), j <= p and (window <= 0, or j > p - window, or j < sinks).
+ *   A row that sees nothing becomes 0, and so does a row at or behind its sequence's end (p >= lengths[b]).  Keys and
+ *   values that a row does not see, whatever they hold, do not reach it.
+ * prefix: keys and values [Hkv, P, D] in front of every sequence, seen by every row that is not behind its sequence's end.
+ * D a multiple of 8 up to 128; pointers 16-byte aligned, strides of q, k, v multiples of 8.
+ * workspace: hbq_attention_workspace_bytes(...) bytes (0: none), 16-byte aligned, contents irrelevant. */
+typedef struct hbq_attention {
+    const void *q, *k, *v;
+    void* out;
+    int64_t B, L, H, Hkv, S, D;
+    int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];   /* q, out: b, l, h;  k, v: b, head, key */
+    const int32_t *lengths, *starts;
+    const void *prefix_k, *prefix_v;
+    int64_t P;
+    int64_t pk_stride[2], pv_stride[2];                             /* head, key */
+    int64_t window, sinks;
+    float scale;
+    int32_t dtype;
+} hbq_attention;
+int hbq_attention_run(const hbq_attention* a, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t hbq_attention_workspace_bytes(const hbq_attention* a);
+
 /* ---- misc ------------------------------------------------------------------------------ */
 
 const char* hbq_error_string(int code);
