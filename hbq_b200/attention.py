@@ -20,8 +20,10 @@ from .rotary import _check_devices, _check_no_gradient, _check_out, _strides, _T
 
 
 def _ready(t: torch.Tensor) -> torch.Tensor:
-    """The tensor as the kernels read it: last axis dense, 16-byte aligned rows; a copy where it is not."""
-    ok = (t.shape[-1] == 1 or t.stride(-1) == 1) and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in _strides(t, 0))
+    """The tensor as the kernels read it: last axis dense, 16-byte aligned rows, every token a row of its own; a copy where it
+    is not."""
+    ok = (t.shape[-1] == 1 or t.stride(-1) == 1) and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in _strides(t, 0)) and \
+        (t.shape[-2] <= 1 or t.stride(-2) > 0)
     return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 

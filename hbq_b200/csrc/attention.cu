@@ -22,10 +22,29 @@ int check(const hbq_attention* p)
     uintptr_t u = reinterpret_cast<uintptr_t>(p->q);
     if (p->S > 0) u |= reinterpret_cast<uintptr_t>(p->k) | reinterpret_cast<uintptr_t>(p->v);
     if (p->P > 0) u |= reinterpret_cast<uintptr_t>(p->prefix_k) | reinterpret_cast<uintptr_t>(p->prefix_v);
-    return (s % 8) || (u & 15) ? HBQ_ERR_ALIGN : HBQ_OK;
+    const bool same_keys = (p->S > 1 && (p->k_stride[2] <= 0 || p->v_stride[2] <= 0)) || (p->P > 1 && (p->pk_stride[1] <= 0 || p->pv_stride[1] <= 0));
+    return (s % 8) || (u & 15) || same_keys ? HBQ_ERR_ALIGN : HBQ_OK;
 }
 
 bool nothing(const hbq_attention* p) { return p->B == 0 || p->L == 0 || p->H == 0; }
+
+// Which kernels a call takes: rows of one token by the warp-level MMA, more rows by the tensor core; the prefix by itself
+// where its rows (of all sequences) are more than the warp-level MMA's 16.
+struct Plan {
+    bool own_tc, prefix_tc;            // prefix_tc: the prefix has a launch of its own, else it is part of the rows' list
+    int own, prefix;                   // pieces
+    int parts() const { return own + prefix; }
+};
+Plan plan_of(const hbq_attention* p)
+{
+    Plan c = {};
+    c.prefix_tc = p->P > 0 && p->B * p->L * (p->H / p->Hkv) > 16;
+    const bool alone = p->P == 0 || c.prefix_tc;
+    c.own_tc = alone && p->L > 1 && p->S > 0;
+    if (c.prefix_tc) c.prefix = attention_tc_parts(p, true);
+    if (!c.prefix_tc || p->S > 0) c.own = c.own_tc ? attention_tc_parts(p, false) : attention_rows_parts(p, !alone);
+    return c;
+}
 
 int64_t part_bytes(const hbq_attention* p, int64_t parts) { return parts > 1 ? p->B * p->L * p->H * parts * (p->D + 2) * 4 : 0; }
 
@@ -33,9 +52,7 @@ int64_t part_bytes(const hbq_attention* p, int64_t parts) { return parts > 1 ? p
 
 int64_t attention_workspace_bytes(const hbq_attention* p)
 {
-    if (check(p) || nothing(p)) return 0;
-    int nsplit;
-    return part_bytes(p, attention_rows_parts(p, &nsplit));
+    return check(p) || nothing(p) ? 0 : part_bytes(p, plan_of(p).parts());
 }
 
 int attention_run(const hbq_attention* p, void* workspace, int64_t workspace_bytes, cudaStream_t stream)
@@ -49,11 +66,22 @@ int attention_run(const hbq_attention* p, void* workspace, int64_t workspace_byt
     a.S = p->S; a.P = p->P; a.window = p->window; a.sinks = p->sinks;
     a.B = (uint32_t)p->B; a.L = (uint32_t)p->L; a.H = (uint32_t)p->H; a.Hkv = (uint32_t)p->Hkv; a.G = (uint32_t)(p->H / p->Hkv); a.D = (uint32_t)p->D;
     a.scale_log2 = p->scale * 1.4426950408889634f;
-    a.parts = (int)attention_rows_parts(p, &a.nsplit);
+    const Plan c = plan_of(p);
+    a.parts = c.parts();
     const int64_t need = part_bytes(p, a.parts);
     if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))) return HBQ_ERR_WORKSPACE;
     a.part = static_cast<float*>(workspace);
-    { const int rc = attention_rows_launch(a, p->dtype, stream); if (rc) return rc; }
+    if (c.prefix_tc) {
+        a.nsplit = c.prefix;
+        { const int rc = attention_tc_launch(a, p->dtype, true, stream); if (rc) return rc; }
+        a.P = 0;
+        a.part0 = c.prefix;
+    }
+    if (c.own) {
+        a.nsplit = c.own;
+        const int rc = c.own_tc ? attention_tc_launch(a, p->dtype, false, stream) : attention_rows_launch(a, p->dtype, stream);
+        if (rc) return rc;
+    }
     return a.parts > 1 ? attention_join_launch(a, p->dtype, stream) : HBQ_OK;
 }
 

@@ -42,6 +42,8 @@ __device__ __forceinline__ float2* part_weight(const AttnArgs& a, int64_t row, i
 
 int attention_join_launch(const AttnArgs& a, int dtype, cudaStream_t stream);                    // attention_rows.cu
 int attention_rows_launch(AttnArgs& a, int dtype, cudaStream_t stream);
-int64_t attention_rows_parts(const hbq_attention* p, int* nsplit);
+int attention_rows_parts(const hbq_attention* p, bool prefix);
+int attention_tc_launch(AttnArgs& a, int dtype, bool prefix, cudaStream_t stream);               // attention_tc.cu
+int attention_tc_parts(const hbq_attention* p, bool prefix);
 
 }  // namespace hbq

@@ -313,20 +313,20 @@ int rows_type(const AttnArgs& a, cudaStream_t stream)
 
 }  // namespace
 
-int64_t attention_rows_parts(const hbq_attention* p, int* nsplit)
+// Into how many pieces a row's list of keys is cut; prefix: the list begins with it.
+int attention_rows_parts(const hbq_attention* p, bool prefix)
 {
     int sms = 148;
     device_sms(&sms);
     const int64_t blocks = p->B * p->L * p->Hkv * ((p->H / p->Hkv + 15) / 16);
     int64_t keys = p->S;
     if (p->window > 0 && p->window + p->sinks < keys) keys = p->window + p->sinks;
-    keys += p->P;
+    if (prefix) keys += p->P;
     // two blocks an SM are resident; twice as many pieces as that even out sequences of different lengths, as far as a
     // piece keeps 128 keys
     int64_t n = ((int64_t)sms * 4 + blocks - 1) / blocks;
     if (n > (keys + 127) / 128) n = (keys + 127) / 128;
-    *nsplit = (int)(n < 1 ? 1 : n > 256 ? 256 : n);
-    return *nsplit;
+    return (int)(n < 1 ? 1 : n > 256 ? 256 : n);
 }
 
 int attention_rows_launch(AttnArgs& a, int dtype, cudaStream_t stream)

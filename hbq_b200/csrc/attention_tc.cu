@@ -1,0 +1,580 @@
+// Attention of many rows against a cache on the tensor core (tcgen05), scores and weights in tensor memory.
+//
+// The G query heads of a key head and the rows of a sequence -- or, against a shared prefix, of all sequences -- form one
+// left operand: row r is token r / G, head r % G.  A block takes 256 of its rows as two tiles of 128 and walks over tiles of
+// 128 keys:  S = Q K^T into tensor memory;  one warpgroup per row tile (thread = row) reads its row of S, masks it, keeps
+// the running maximum and sum of a softmax and writes the weights back over S in the values' type;  O += P V with P from tensor
+// memory.  While one warpgroup works on its tile's scores the tensor core multiplies for the other.
+// O stays in tensor memory; its rows are rescaled only when a row's maximum has grown by more than 2^8 in the weights
+// since the last time (weights up to 2^12 are as exact as weights up to 1, and the sum divides the factor out again).
+//
+// Keys come by TMA in a ring that keys and values share, from a cache of any strides.  Tiles that the masks of all rows hide
+// are left out; the mask is applied only in tiles that hide some key from some row.  There the weights hold zeros, and a
+// zero times an infinity or a NaN of a hidden value would still reach the sum: such values are set to zero in shared memory
+// before the product, and the rows that do see them get them added at the end.
+#include "attention_dev.cuh"
+#include "tc_dev.cuh"
+
+namespace hbq {
+
+namespace {
+
+constexpr int TILE = 128, TCT = 320;
+constexpr uint32_t POLLS = 1u << 20;
+constexpr float SHIFT = 4.f;           // weights are 2^(x - maximum + 4): in fp16 that keeps 16 times smaller ones normal
+constexpr float GROWTH = 8.f;          // in powers of two; 2^(4 + 8) stays below fp16's largest
+
+template <int DP> struct TcShape {
+    static constexpr int HALVES = DP / 64;
+    static constexpr int STAGE = TILE * DP * 2, Q = 2 * TILE * DP * 2;
+    static constexpr int NS = DP == 128 ? 5 : 8;
+    static constexpr int BYTES = 1024 + Q + NS * STAGE + 256;
+};
+
+struct TcTask {
+    uint32_t R;                        // rows of a key head: L * G, or B * L * G against a prefix
+    uint32_t groups;                   // sequences with keys of their own: B, or 1
+    uint32_t tiles;                    // row tiles of 256
+    int prefix, k_by_head, k_by_seq, v_by_head, v_by_seq, vector_out;
+};
+
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code)
+{
+    #pragma unroll 1
+    for (uint32_t it = 0; it < POLLS; ++it) {
+        if (__all_sync(0xFFFFFFFFu, mbar_try_wait(bar, parity))) return true;
+        if ((it & 63u) == 63u && __any_sync(0xFFFFFFFFu, *abort_flag != 0)) return false;
+    }
+    if ((threadIdx.x & 31) == 0) { *abort_flag = 1; atomicCAS(&g_tc_status, 0, code); }
+    __syncwarp();
+    return false;
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+// Values [keys][64 columns of a head] with 128-byte rows and 128-byte swizzle, as the right operand whose rows are keys
+// (the contraction): 8 keys 1024 B apart, 64 columns one half tile apart.
+__device__ __forceinline__ uint64_t values_desc(uint32_t saddr)
+{
+    constexpr uint32_t kHi = 64u | (1u << 14) | (2u << 29);
+    constexpr uint32_t kLbo = (TILE * 128) >> 4;
+    return ((uint64_t)kHi << 32) | ((saddr & 0x3FFFFu) >> 4) | (kLbo << 16);
+}
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t* r)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+                 "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void tc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void add2(float& d0, float& d1, float a0, float a1)
+{
+    asm("{ .reg .b64 ra, rb;\n mov.b64 ra, {%0, %1};\n mov.b64 rb, {%2, %3};\n add.rn.f32x2 ra, ra, rb;\n mov.b64 {%0, %1}, ra; }"
+        : "+f"(d0), "+f"(d1) : "f"(a0), "f"(a1));
+}
+
+template <class E> struct Word;
+template <> struct Word<__half> {
+    static constexpr uint32_t FORMAT = 0, INF = 0x7C00u;
+    static __device__ __forceinline__ uint32_t pack(float a, float b) { return h2_bits(__floats2half2_rn(a, b)); }
+    static __device__ __forceinline__ float up(uint16_t u) { return __half2float(bits_h(u)); }
+};
+template <> struct Word<__nv_bfloat16> {
+    static constexpr uint32_t FORMAT = 1, INF = 0x7F80u;
+    static __device__ __forceinline__ uint32_t pack(float a, float b)
+    {
+        __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ float up(uint16_t u) { return __uint_as_float((uint32_t)u << 16); }
+};
+
+// What the rows of a block see, in key positions: all rows that see anything stand between pa and pb.
+struct Span {
+    int pa, pb, window, sinks;         // window: 0 for none
+    int first_tiles, low_tile;         // list of key tiles: the first `first_tiles` ones, then those from low_tile on
+    int count;
+    __device__ __forceinline__ int tile(int u) const { return u < first_tiles ? u : low_tile + u - first_tiles; }
+    // every key of the tile is seen by every row between pa and pb
+    __device__ __forceinline__ bool whole(int j0) const
+    {
+        return j0 + TILE - 1 <= pa && (window == 0 || j0 > pb - window || j0 + TILE - 1 < sinks);
+    }
+    __device__ __forceinline__ bool seen_by_some(int j) const { return j <= pb && (window == 0 || j > pa - window || j < sinks); }
+};
+
+template <class E, int DP>
+__global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                              const __grid_constant__ AttnArgs a, const __grid_constant__ TcTask task)
+{
+    using Sh = TcShape<DP>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+    const uint32_t qs = base, ring = base + Sh::Q, ctrl = ring + Sh::NS * Sh::STAGE;
+    uint8_t* ctrl_p = smem_raw + (ctrl - raw);
+    const uint32_t kv_full = ctrl, kv_empty = ctrl + 8 * Sh::NS, q_full = ctrl + 16 * Sh::NS;
+    const uint32_t s_full = q_full + 8, p_ready = q_full + 24, o_full = q_full + 40;        // two each
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ctrl_p + 16 * Sh::NS + 64);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(ctrl_p + 16 * Sh::NS + 72);
+    volatile int* special = reinterpret_cast<volatile int*>(ctrl_p + 16 * Sh::NS + 76);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < Sh::NS; ++s) { mbar_init(kv_full + 8 * s, 1); mbar_init(kv_empty + 8 * s, 1); }
+        mbar_init(q_full, 8);
+        for (int t = 0; t < 2; ++t) { mbar_init(s_full + 8 * t, 1); mbar_init(p_ready + 8 * t, 4); mbar_init(o_full + 8 * t, 1); }
+        *abort_flag = 0;
+        *special = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    grid_dependency_wait();
+    dependents_may_start();
+    const uint32_t tmem = *tmem_slot;
+
+    // this block: rows r0 .. r0 + 255 of key head hk of a sequence (group), a piece of their keys; the rows that see the
+    // most keys first, so that the last blocks to start are short ones
+    uint32_t id = blockIdx.x;
+    const uint32_t split = id % (uint32_t)a.nsplit; id /= (uint32_t)a.nsplit;
+    const uint32_t hk = id % a.Hkv; id /= a.Hkv;
+    const uint32_t group = id % task.groups;
+    const uint32_t r0 = (task.tiles - 1 - id / task.groups) * 256u, rend = min(r0 + 256u, task.R);
+    const bool two = r0 + TILE < task.R;
+
+    int64_t n64 = 0, first = 0;
+    Span sp = {};
+    sp.sinks = (int)min(a.sinks, (int64_t)0x7FFFFFFF);
+    if (task.prefix) {
+        sp.pa = sp.pb = (int)a.P - 1;
+        sp.count = (int)((a.P + TILE - 1) / TILE);
+    } else {
+        sequence_of(a, group, &n64, &first);
+        const int64_t p0 = first + r0 / a.G, p1 = first + (rend - 1) / a.G;
+        const int64_t pa = p0 > 0 ? p0 : 0, pb = p1 < n64 - 1 ? p1 : n64 - 1;
+        if (pa <= pb) {
+            sp.pa = (int)pa; sp.pb = (int)pb;
+            sp.window = a.window > 0 && a.window <= pb ? (int)a.window : 0;
+            const int low = sp.window && sp.pa - sp.window + 1 > 0 ? sp.pa - sp.window + 1 : 0;
+            sp.low_tile = low / TILE;
+            const int st = sp.window ? (sp.sinks >= low ? sp.low_tile : (sp.sinks + TILE - 1) / TILE) : 0;
+            sp.first_tiles = min(st, sp.low_tile);
+            sp.count = sp.first_tiles + sp.pb / TILE - sp.low_tile + 1;
+        }
+    }
+    const int u0 = (int)((int64_t)sp.count * split / a.nsplit), u1 = (int)((int64_t)sp.count * (split + 1) / a.nsplit), nt = u1 - u0;
+
+    if (warp == 9) {
+        // ================= keys and values =================
+        if (lane == 0 && nt > 0) {
+            const int kh = task.k_by_head ? (int)hk : 0, kb = task.k_by_seq ? (int)group : 0;
+            const int vh = task.v_by_head ? (int)hk : 0, vb = task.v_by_seq ? (int)group : 0;
+            uint32_t stage = 0, phase = 1;
+            bool ok = true;
+            for (int x = 0; x < 2 * nt && ok; ++x) {
+                if (!(ok = mbar_wait(kv_empty + 8 * stage, phase, abort_flag, 41, POLLS))) break;
+                const int j0 = sp.tile(u0 + (x >> 1)) * TILE;
+                const uint32_t dst = ring + stage * Sh::STAGE, bar = kv_full + 8 * stage;
+                mbar_expect_tx(bar, Sh::STAGE);
+                #pragma unroll
+                for (int h = 0; h < Sh::HALVES; ++h) {
+                    if (x & 1) tma_load_4d(dst + h * (TILE * 128), &map_v, h * 64, j0, vh, vb, bar);
+                    else tma_load_4d(dst + h * (TILE * 128), &map_k, h * 64, j0, kh, kb, bar);
+                }
+                if (++stage == Sh::NS) { stage = 0; phase ^= 1u; }
+            }
+        }
+    } else if (warp == 8) {
+        // ================= products =================
+        if (nt > 0) {
+            constexpr uint32_t S_IDESC = (1u << 4) | (Word<E>::FORMAT << 7) | (Word<E>::FORMAT << 10) | ((TILE >> 3) << 17) | ((TILE >> 4) << 24);
+            constexpr uint32_t O_IDESC = (1u << 4) | (Word<E>::FORMAT << 7) | (Word<E>::FORMAT << 10) | (1u << 16) | ((DP >> 3) << 17) | ((TILE >> 4) << 24);
+            const bool leader = elect_one();
+            auto scores = [&](int t, uint32_t stage) {
+                if (leader) {
+                    const uint32_t ka = ring + stage * Sh::STAGE, qa = qs + t * (TILE * 128);
+                    #pragma unroll
+                    for (int kk = 0; kk < DP / 16; ++kk)
+                        tc_mma_f16(tmem + t * TILE, umma_desc(qa + (kk >> 2) * (2 * TILE * 128) + (kk & 3) * 32),
+                                   umma_desc(ka + (kk >> 2) * (TILE * 128) + (kk & 3) * 32), S_IDESC, kk != 0);
+                    tc_commit(s_full + 8 * t);
+                }
+            };
+            auto output = [&](int t, uint32_t stage, bool more) {
+                if (leader) {
+                    const uint32_t va = ring + stage * Sh::STAGE;
+                    #pragma unroll
+                    for (int kk = 0; kk < TILE / 16; ++kk)
+                        mma_ts(tmem + 2 * TILE + t * DP, tmem + t * TILE + kk * 8, values_desc(va + kk * 2048), O_IDESC, more || kk != 0);
+                }
+            };
+            uint32_t ks = 0, kph = 0;                       // stage and phase of the next ring entry
+            auto next = [&] { if (++ks == Sh::NS) { ks = 0; kph ^= 1u; } };
+            bool ok = wait_for(q_full, 0, abort_flag, 42) && wait_for(kv_full + 8 * ks, kph, abort_flag, 43);
+            if (ok) {
+                tc_fence_after();
+                scores(0, ks);
+                if (two) scores(1, ks);
+                if (leader) tc_commit(kv_empty + 8 * ks);
+                next();
+            }
+            for (int j = 0; j < nt && ok; ++j) {
+                const uint32_t vs = ks, par = (uint32_t)j & 1u;
+                const bool more = j + 1 < nt;
+                if (!(ok = wait_for(kv_full + 8 * ks, kph, abort_flag, 43))) break;
+                next();
+                if (!(ok = wait_for(p_ready, par, abort_flag, 44))) break;
+                tc_fence_after();
+                output(0, vs, j > 0);
+                if (more) {
+                    if (!(ok = wait_for(kv_full + 8 * ks, kph, abort_flag, 43))) break;
+                    tc_fence_after();
+                    scores(0, ks);
+                } else if (leader) tc_commit(o_full);
+                if (two) {
+                    if (!(ok = wait_for(p_ready + 8, par, abort_flag, 44))) break;
+                    tc_fence_after();
+                    output(1, vs, j > 0);
+                }
+                if (leader) tc_commit(kv_empty + 8 * vs);
+                if (more) {
+                    if (two) scores(1, ks);
+                    if (leader) tc_commit(kv_empty + 8 * ks);
+                    next();
+                } else if (two && leader) tc_commit(o_full + 8);
+            }
+        }
+    } else {
+        // ================= rows =================
+        const int t = warp >> 2, wr = (warp & 3) * 32 + lane;
+        const uint32_t r = r0 + t * TILE + wr;
+        uint32_t b = group, i = 0, h = 0;
+        int hi = -1, lo = 0;                                 // this row sees keys lo .. hi and those before sp.sinks
+        if (r < rend) {
+            uint32_t rr = r;
+            if (task.prefix) { b = rr / (a.L * a.G); rr -= b * (a.L * a.G); }
+            i = rr / a.G;
+            h = hk * a.G + (rr - i * a.G);
+            if (task.prefix) sequence_of(a, b, &n64, &first);
+            const int64_t p = first + i;
+            if (p < n64) {
+                if (task.prefix) hi = (int)a.P - 1;
+                else if (p >= 0) {
+                    hi = (int)p;
+                    lo = sp.window ? (int)p - sp.window + 1 : 0;
+                }
+            }
+        }
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t s_col = lanes + t * TILE, o_col = lanes + 2 * TILE + t * DP;
+        bool ok = true;
+        float m = -INFINITY, l = 0.f;
+        const float c = a.scale_log2;
+        if (nt > 0) {
+            // queries of this warp's 32 rows: 16-byte pieces, neighbouring lanes along a row
+            constexpr int PIECES = DP / 8;
+            #pragma unroll 4
+            for (int x = lane; x < 32 * PIECES; x += 32) {
+                const int row = x / PIECES, pc = x - row * PIECES;
+                const uint32_t q = warp * 32 + row, at = r0 + q;
+                uint4 u = make_uint4(0, 0, 0, 0);
+                if (at < rend && pc * 8 < (int)a.D) {
+                    uint32_t rr = at, bb = group;
+                    if (task.prefix) { bb = rr / (a.L * a.G); rr -= bb * (a.L * a.G); }
+                    const uint32_t ii = rr / a.G, hh = hk * a.G + (rr - ii * a.G);
+                    u = *reinterpret_cast<const uint4*>(static_cast<const E*>(a.q) + (int64_t)bb * a.qs[0] + (int64_t)ii * a.qs[1] + (int64_t)hh * a.qs[2] + pc * 8);
+                }
+                const uint32_t dst = qs + (pc >> 3) * (2 * TILE * 128) + q * 128 + (((pc & 7) ^ (q & 7)) * 16);
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+        }
+        uint32_t vs = 1, vph = 0;                            // ring entry of this step's values
+        if (t == 0 || two)
+        for (int u = 0; u < nt; ++u) {
+            if (!(ok = wait_for(s_full + 8 * t, (uint32_t)u & 1u, abort_flag, 45))) break;
+            tc_fence_after();
+            uint32_t s[128];
+            #pragma unroll
+            for (int k = 0; k < 4; ++k) tc_ld32_issue(s_col + 32 * k, s + 32 * k);
+            tc_ld_wait(s);
+            #pragma unroll
+            for (int k = 1; k < 4; ++k) tc_ld_landed(s + 32 * k);
+            const int j0 = sp.tile(u0 + u) * TILE;
+            const bool whole = sp.whole(j0);
+            if (!whole) {
+                const int top = hi - j0, low = lo - j0, sink = sp.sinks - j0;
+                #pragma unroll
+                for (int k = 0; k < 128; ++k)
+                    if (k > top || (k < low && k >= sink)) s[k] = 0xFF800000u;
+            }
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            #pragma unroll
+            for (int k = 0; k < 128; ++k) mx[k & 3] = fmaxf(mx[k & 3], __uint_as_float(s[k]));
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            const bool grow = (top - m) * c > GROWTH;        // (from -inf: any; -inf itself: NaN, false)
+            if (__any_sync(0xFFFFFFFFu, grow)) {
+                const float f = grow ? exp2_fast((m - top) * c) : 1.f;
+                if (grow) m = top;
+                l *= f;
+                if (u > 0) {
+                    #pragma unroll 1
+                    for (int k = 0; k < DP / 16; ++k) {
+                        uint32_t o[16];
+                        asm volatile(
+                            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+                            "tcgen05.wait::ld.sync.aligned;"
+                            : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]), "=r"(o[4]), "=r"(o[5]), "=r"(o[6]), "=r"(o[7]), "=r"(o[8]),
+                              "=r"(o[9]), "=r"(o[10]), "=r"(o[11]), "=r"(o[12]), "=r"(o[13]), "=r"(o[14]), "=r"(o[15]) : "r"(o_col + 16 * k) : "memory");
+                        #pragma unroll
+                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tc_st16(o_col + 16 * k, o);
+                    }
+                }
+            }
+            const float off = SHIFT - (m == -INFINITY ? 0.f : m * c);
+            float sum[4] = {};
+            #pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                uint32_t w[16];
+                #pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    float x, y;
+                    fma2(x, y, __uint_as_float(s[32 * q + 2 * k]), __uint_as_float(s[32 * q + 2 * k + 1]), c, off);
+                    x = exp2_fast(x); y = exp2_fast(y);
+                    add2(sum[2 * (k & 1)], sum[2 * (k & 1) + 1], x, y);
+                    w[k] = Word<E>::pack(x, y);
+                }
+                tc_st16(s_col + 16 * q, w);
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            if (!whole && t == 0) {
+                // infinities and NaNs among this tile's values: thread = key
+                if (!(ok = wait_for(kv_full + 8 * vs, vph, abort_flag, 46))) break;
+                const uint32_t row = ring + vs * Sh::STAGE + wr * 128;
+                bool found = false;
+                #pragma unroll 4
+                for (int pc = 0; pc < DP / 8; ++pc) {
+                    const uint32_t at = row + (pc >> 3) * (TILE * 128) + (((pc & 7) ^ (wr & 7)) * 16);
+                    uint32_t x[4];
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at) : "memory");
+                    constexpr uint32_t LOW = Word<E>::INF, HIGH = Word<E>::INF << 16;
+                    bool bad = false;
+                    #pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const bool b0 = (x[e] & LOW) == LOW, b1 = (x[e] & HIGH) == HIGH;
+                        bad |= b0 || b1;
+                        if (b0) x[e] &= 0xFFFF0000u;
+                        if (b1) x[e] &= 0x0000FFFFu;
+                    }
+                    if (bad) {
+                        found = true;
+                        if (sp.seen_by_some(j0 + wr)) { *special = 1; __threadfence_block(); }
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+                    }
+                }
+                if (found) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            }
+            vs += 2;
+            if (vs >= Sh::NS) { vs -= Sh::NS; vph ^= 1u; }
+            tc_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_ready + 8 * t);
+        }
+        // ---- the rows' results ----
+        if (ok && (t == 0 || two)) {
+            if (nt > 0) ok = wait_for(o_full + 8 * t, 0, abort_flag, 47);
+            tc_fence_after();
+            const bool direct = a.parts == 1, add = nt > 0 && *special;
+            const bool live = hi >= 0 && l != 0.f;            // (a NaN counts as something)
+            const float f = direct ? (live ? 1.f / l : 0.f) : 1.f;
+            const int64_t row = ((int64_t)b * a.L + i) * a.H + h;
+            E* out = static_cast<E*>(a.out) + (int64_t)b * a.os[0] + (int64_t)i * a.os[1] + (int64_t)h * a.os[2];
+            float* part = direct ? nullptr : part_sum(a, row, a.part0 + split);
+            if (ok) {
+                #pragma unroll 1
+                for (int k = 0; k < DP / 32; ++k) {
+                    float o[32];
+                    __syncwarp();
+                    if (nt > 0) tc_ld32(o_col + 32 * k, o);
+                    if (!live) {
+                        #pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = 0.f;
+                    }
+                    if (add && live) {
+                        const E* v = task.prefix ? static_cast<const E*>(a.pv) + (int64_t)hk * a.pvs[0]
+                                                 : static_cast<const E*>(a.v) + (int64_t)group * a.vs[0] + (int64_t)hk * a.vs[1];
+                        const int64_t vstep = task.prefix ? a.pvs[1] : a.vs[2];
+                        for (int u = u0; u < u1; ++u) {
+                            const int j0 = sp.tile(u) * TILE;
+                            if (sp.whole(j0)) continue;
+                            for (int j = j0; j < j0 + TILE && j <= hi; ++j) {
+                                if (j < lo && j >= sp.sinks) continue;
+                                #pragma unroll 1
+                                for (int e = 0; e < 32; ++e) {
+                                    if (32 * k + e >= (int)a.D) break;
+                                    const float x = Word<E>::up(reinterpret_cast<const uint16_t*>(v)[j * vstep + 32 * k + e]);
+                                    if (!isfinite(x)) {
+                                        #pragma unroll
+                                        for (int z = 0; z < 32; ++z) if (z == e) o[z] += x;
+                                    }
+                                }
+                            }
+                        }
+                    }
+                    if (r >= rend) {
+                    } else if (direct) {
+                        #pragma unroll
+                        for (int e = 0; e < 32; e += 8) {
+                            if (32 * k + e < (int)a.D) {
+                                uint32_t w[4];
+                                #pragma unroll
+                                for (int z = 0; z < 4; ++z) w[z] = Word<E>::pack(o[e + 2 * z] * f, o[e + 2 * z + 1] * f);
+                                if (task.vector_out) *reinterpret_cast<uint4*>(out + 32 * k + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                                else {
+                                    #pragma unroll
+                                    for (int z = 0; z < 8; ++z) reinterpret_cast<uint16_t*>(out)[32 * k + e + z] = (uint16_t)(w[z >> 1] >> (16 * (z & 1)));
+                                }
+                            }
+                        }
+                    } else {
+                        #pragma unroll
+                        for (int e = 0; e < 32; e += 4)
+                            if (32 * k + e < (int)a.D) *reinterpret_cast<float4*>(part + 32 * k + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    }
+                }
+                if (!direct && r < rend)
+                    *part_weight(a, row, a.part0 + split) = live ? make_float2((m == -INFINITY ? 0.f : m * c) - SHIFT, l) : make_float2(-INFINITY, 0.f);
+            }
+        }
+    }
+
+    // ---- teardown: every role arrives here, also after an expired wait ----
+    tc_fence_before();
+    __syncthreads();
+    if (*abort_flag) {
+        // let copies that may still be in flight land before the block's shared memory is released
+        const unsigned long long t0 = gtime_ns();
+        while (gtime_ns() - t0 < 200000ull) { }
+        __syncthreads();
+    }
+    if (warp == 8) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                             const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encoder()
+{
+    static EncodeFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult qr;
+        const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qr) == cudaSuccess && qr == cudaDriverEntryPointSuccess;
+        return ok ? (EncodeFn)p : (EncodeFn) nullptr;
+    }();
+    return fn;
+}
+
+// A cache [sequences][heads][keys][D] in boxes of 128 keys by 64 values; keys beyond the last and values beyond D read as
+// zeros.  An axis whose elements are all the same ones (stride 0) is left out.
+int cache_map(CUtensorMap* map, const void* ptr, int dtype, int64_t D, int64_t keys, int64_t key_stride, int64_t heads, int64_t head_stride,
+              int64_t seqs, int64_t seq_stride)
+{
+    EncodeFn fn = encoder();
+    if (!fn) return HBQ_ERR_CUDA;
+    const auto step = [](int64_t stride, int64_t other) { return (cuuint64_t)(stride > 0 ? stride : other) * 2; };
+    const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)keys, (cuuint64_t)(head_stride > 0 ? heads : 1), (cuuint64_t)(seq_stride > 0 ? seqs : 1)};
+    const cuuint64_t strides[3] = {step(key_stride, D), step(head_stride, D), step(seq_stride, D)};
+    const cuuint32_t box[4] = {64, TILE, 1, 1}, each[4] = {1, 1, 1, 1};
+    const CUresult r = fn(map, dtype == HBQ_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr), dims,
+                          strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? HBQ_OK : HBQ_ERR_CUDA;
+}
+
+template <class E, int DP>
+int tc_launch(const CUtensorMap& mk, const CUtensorMap& mv, const AttnArgs& a, const TcTask& task, unsigned blocks, cudaStream_t stream)
+{
+    { const int rc = ensure_dynamic_smem(attention_tc_kernel<E, DP>, TcShape<DP>::BYTES); if (rc) return rc; }
+    HBQ_CUDA_TRY(launch_dependent(attention_tc_kernel<E, DP>, blocks, TCT, (size_t)TcShape<DP>::BYTES, stream, mk, mv, a, task));
+    HBQ_LAUNCH_CHECK("attention_tc_kernel");
+    return HBQ_OK;
+}
+
+}  // namespace
+
+// Into how many pieces the keys of a block's rows are cut: the count with the shortest longest SM, where a block costs its
+// key tiles and about three tiles' time to start and end, and joining pieces about four.
+int attention_tc_parts(const hbq_attention* p, bool prefix)
+{
+    int sms = 148;
+    device_sms(&sms);
+    const int64_t G = p->H / p->Hkv, R = (prefix ? p->B : 1) * p->L * G, blocks = (R + 255) / 256 * p->Hkv * (prefix ? 1 : p->B);
+    int64_t keys = prefix ? p->P : p->S;
+    if (!prefix && p->window > 0 && p->window + p->sinks + 256 / G + 256 < keys) keys = p->window + p->sinks + 256 / G + 256;
+    const int64_t tiles = (keys + TILE - 1) / TILE;
+    int64_t best = 1, cost = (blocks + sms - 1) / sms * (tiles + 3);
+    for (int64_t n = 2; n <= 64 && n <= tiles && blocks * n <= 2 * sms; ++n) {
+        const int64_t now = (blocks * n + sms - 1) / sms * ((tiles + n - 1) / n + 3) + 4;
+        if (now < cost) { cost = now; best = n; }
+    }
+    return (int)best;
+}
+
+// The rows of `a` against their own keys, or (prefix) all sequences' rows against the prefix.
+int attention_tc_launch(AttnArgs& a, int dtype, bool prefix, cudaStream_t stream)
+{
+    TcTask task = {};
+    const int64_t R = (int64_t)(prefix ? a.B : 1) * a.L * a.G;
+    if (R > 0x7FFFFF00ll) return HBQ_ERR_UNSUPPORTED;
+    task.R = (uint32_t)R; task.groups = prefix ? 1 : a.B; task.tiles = (task.R + 255) / 256; task.prefix = prefix;
+    const int64_t blocks = (int64_t)task.tiles * task.groups * a.Hkv * a.nsplit;
+    if (blocks > 0x7FFFFFFFll) return HBQ_ERR_UNSUPPORTED;
+    const int64_t pks[3] = {0, a.pks[0], a.pks[1]}, pvs[3] = {0, a.pvs[0], a.pvs[1]};
+    const int64_t *ks = prefix ? pks : a.ks, *vs = prefix ? pvs : a.vs;
+    task.k_by_seq = ks[0] > 0; task.k_by_head = ks[1] > 0; task.v_by_seq = vs[0] > 0; task.v_by_head = vs[1] > 0;
+    task.vector_out = ((a.os[0] | a.os[1] | a.os[2]) % 8) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+    CUtensorMap mk, mv;
+    const int64_t keys = prefix ? a.P : a.S;
+    { const int rc = cache_map(&mk, prefix ? a.pk : a.k, dtype, a.D, keys, ks[2], a.Hkv, ks[1], a.B, ks[0]); if (rc) return rc; }
+    { const int rc = cache_map(&mv, prefix ? a.pv : a.v, dtype, a.D, keys, vs[2], a.Hkv, vs[1], a.B, vs[0]); if (rc) return rc; }
+    const bool wide = a.D > 64;
+    if (dtype == HBQ_DTYPE_F16)
+        return wide ? tc_launch<__half, 128>(mk, mv, a, task, (unsigned)blocks, stream) : tc_launch<__half, 64>(mk, mv, a, task, (unsigned)blocks, stream);
+    return wide ? tc_launch<__nv_bfloat16, 128>(mk, mv, a, task, (unsigned)blocks, stream)
+                : tc_launch<__nv_bfloat16, 64>(mk, mv, a, task, (unsigned)blocks, stream);
+}
+
+int attention_tc_status(int* host_out)
+{
+    HBQ_CUDA_TRY(cudaMemcpyFromSymbol(host_out, g_tc_status, sizeof(int)));
+    return HBQ_OK;
+}
+int attention_tc_status_reset()
+{
+    const int z = 0;
+    HBQ_CUDA_TRY(cudaMemcpyToSymbol(g_tc_status, &z, sizeof(int)));
+    return HBQ_OK;
+}
+
+}  // namespace hbq

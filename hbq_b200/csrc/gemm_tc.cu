@@ -741,21 +741,27 @@ int gemm_tc_reserve_sms(int n)
 
 int gemm_w4_status(int* host_out);          // gemm_packed.cu: that kernel's own status word
 int gemm_w4_status_reset();
+int attention_tc_status(int* host_out);     // attention_tc.cu: likewise
+int attention_tc_status_reset();
 
-// Non-zero when a wait gave up in either tensor-core kernel (the packed-weight kernel's codes are offset by 16).
+// Non-zero when a wait gave up in any tensor-core kernel (the packed-weight kernel's codes are offset by 16, the attention
+// kernel's begin at 41).
 int gemm_tc_status(int* host_out)
 {
     int s = 0, p = 0;
     HBQ_CUDA_TRY(cudaMemcpyFromSymbol(&s, g_tc_status, sizeof(int)));
     { const int rc = gemm_w4_status(&p); if (rc) return rc; }
-    *host_out = s ? s : (p ? 16 + p : 0);
+    int t = 0;
+    { const int rc = attention_tc_status(&t); if (rc) return rc; }
+    *host_out = s ? s : p ? 16 + p : t;
     return HBQ_OK;
 }
 int gemm_tc_status_reset()
 {
     const int z = 0;
     HBQ_CUDA_TRY(cudaMemcpyToSymbol(g_tc_status, &z, sizeof(int)));
-    return gemm_w4_status_reset();
+    { const int rc = gemm_w4_status_reset(); if (rc) return rc; }
+    return attention_tc_status_reset();
 }
 
 }  // namespace hbq
