@@ -38,6 +38,19 @@ struct TcTask {
     int prefix, k_by_head, k_by_seq, v_by_head, v_by_seq, vector_out;
 };
 
+// Bounded wait of one thread, and of a warp by its lane 0 (a poll by all lanes is 32 accesses to the barrier's word, beside
+// the tensor core's own use of shared memory).
+__device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code)
+{
+    #pragma unroll 1
+    for (uint32_t it = 0; it < POLLS; ++it) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((it & 63u) == 63u && *abort_flag) return false;
+    }
+    *abort_flag = 1;
+    atomicCAS(&g_tc_status, 0, code);
+    return false;
+}
 __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code)
 {
     #pragma unroll 1
@@ -81,6 +94,27 @@ __device__ __forceinline__ void add2(float& d0, float& d1, float a0, float a1)
 {
     asm("{ .reg .b64 ra, rb;\n mov.b64 ra, {%0, %1};\n mov.b64 rb, {%2, %3};\n add.rn.f32x2 ra, ra, rb;\n mov.b64 {%0, %1}, ra; }"
         : "+f"(d0), "+f"(d1) : "f"(a0), "f"(a1));
+}
+
+// Two powers of two on the FMA pipe (the special-function unit alone would take as long as the products): x = n + f with
+// n the nearest whole number, 2^f by a polynomial on [-1/2, 1/2] (minimax in the relative error, 2.7e-6), 2^n from its bits.
+// n is at least -127, whose bits are those of 0; a NaN stays one.
+__device__ __forceinline__ void exp2_pair(float& x, float& y)
+{
+    constexpr float MAGIC = 12582912.f + 127.f;                // 1.5 * 2^23: the sum's last bits are n + 127
+    constexpr float C0 = 0.9999992847f, C1 = 0.6931217909f, C2 = 0.2402474433f, C3 = 0.0559178628f, C4 = 0.00957010221f;
+    float t0, t1, p0, p1;
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-127.f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(y) : "f"(-127.f));
+    asm("{ .reg .b64 x, t, r, f, p, k;\n"
+        " mov.b64 x, {%4, %5};\n mov.b64 k, {%6, %6};\n add.rn.f32x2 t, x, k;\n mov.b64 {%0, %1}, t;\n"
+        " mov.b64 k, {%7, %7};\n add.rn.f32x2 r, t, k;\n mov.b64 k, {%8, %8};\n fma.rn.f32x2 f, r, k, x;\n"
+        " mov.b64 p, {%9, %9};\n mov.b64 k, {%10, %10};\n fma.rn.f32x2 p, p, f, k;\n mov.b64 k, {%11, %11};\n fma.rn.f32x2 p, p, f, k;\n"
+        " mov.b64 k, {%12, %12};\n fma.rn.f32x2 p, p, f, k;\n mov.b64 k, {%13, %13};\n fma.rn.f32x2 p, p, f, k;\n mov.b64 {%2, %3}, p; }"
+        : "=&f"(t0), "=&f"(t1), "=&f"(p0), "=&f"(p1)
+        : "f"(x), "f"(y), "f"(MAGIC), "f"(-MAGIC), "f"(-1.f), "f"(C4), "f"(C3), "f"(C2), "f"(C1), "f"(C0));
+    x = p0 * __uint_as_float(__float_as_uint(t0) << 23);
+    y = p1 * __uint_as_float(__float_as_uint(t1) << 23);
 }
 
 template <class E> struct Word;
@@ -187,7 +221,7 @@ __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_const
             uint32_t stage = 0, phase = 1;
             bool ok = true;
             for (int x = 0; x < 2 * nt && ok; ++x) {
-                if (!(ok = mbar_wait(kv_empty + 8 * stage, phase, abort_flag, 41, POLLS))) break;
+                if (!(ok = wait_one(kv_empty + 8 * stage, phase, abort_flag, 41))) break;
                 const int j0 = sp.tile(u0 + (x >> 1)) * TILE;
                 const uint32_t dst = ring + stage * Sh::STAGE, bar = kv_full + 8 * stage;
                 mbar_expect_tx(bar, Sh::STAGE);
@@ -201,62 +235,57 @@ __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_const
         }
     } else if (warp == 8) {
         // ================= products =================
-        if (nt > 0) {
+        if (nt > 0 && elect_one()) {
             constexpr uint32_t S_IDESC = (1u << 4) | (Word<E>::FORMAT << 7) | (Word<E>::FORMAT << 10) | ((TILE >> 3) << 17) | ((TILE >> 4) << 24);
             constexpr uint32_t O_IDESC = (1u << 4) | (Word<E>::FORMAT << 7) | (Word<E>::FORMAT << 10) | (1u << 16) | ((DP >> 3) << 17) | ((TILE >> 4) << 24);
-            const bool leader = elect_one();
             auto scores = [&](int t, uint32_t stage) {
-                if (leader) {
-                    const uint32_t ka = ring + stage * Sh::STAGE, qa = qs + t * (TILE * 128);
-                    #pragma unroll
-                    for (int kk = 0; kk < DP / 16; ++kk)
-                        tc_mma_f16(tmem + t * TILE, umma_desc(qa + (kk >> 2) * (2 * TILE * 128) + (kk & 3) * 32),
-                                   umma_desc(ka + (kk >> 2) * (TILE * 128) + (kk & 3) * 32), S_IDESC, kk != 0);
-                    tc_commit(s_full + 8 * t);
-                }
+                const uint32_t ka = ring + stage * Sh::STAGE, qa = qs + t * (TILE * 128);
+                #pragma unroll
+                for (int kk = 0; kk < DP / 16; ++kk)
+                    tc_mma_f16(tmem + t * TILE, umma_desc(qa + (kk >> 2) * (2 * TILE * 128) + (kk & 3) * 32),
+                               umma_desc(ka + (kk >> 2) * (TILE * 128) + (kk & 3) * 32), S_IDESC, kk != 0);
+                tc_commit(s_full + 8 * t);
             };
             auto output = [&](int t, uint32_t stage, bool more) {
-                if (leader) {
-                    const uint32_t va = ring + stage * Sh::STAGE;
-                    #pragma unroll
-                    for (int kk = 0; kk < TILE / 16; ++kk)
-                        mma_ts(tmem + 2 * TILE + t * DP, tmem + t * TILE + kk * 8, values_desc(va + kk * 2048), O_IDESC, more || kk != 0);
-                }
+                const uint32_t va = ring + stage * Sh::STAGE;
+                #pragma unroll
+                for (int kk = 0; kk < TILE / 16; ++kk)
+                    mma_ts(tmem + 2 * TILE + t * DP, tmem + t * TILE + kk * 8, values_desc(va + kk * 2048), O_IDESC, more || kk != 0);
             };
             uint32_t ks = 0, kph = 0;                       // stage and phase of the next ring entry
             auto next = [&] { if (++ks == Sh::NS) { ks = 0; kph ^= 1u; } };
-            bool ok = wait_for(q_full, 0, abort_flag, 42) && wait_for(kv_full + 8 * ks, kph, abort_flag, 43);
+            bool ok = wait_one(q_full, 0, abort_flag, 42) && wait_one(kv_full + 8 * ks, kph, abort_flag, 43);
             if (ok) {
                 tc_fence_after();
                 scores(0, ks);
                 if (two) scores(1, ks);
-                if (leader) tc_commit(kv_empty + 8 * ks);
+                tc_commit(kv_empty + 8 * ks);
                 next();
             }
             for (int j = 0; j < nt && ok; ++j) {
                 const uint32_t vs = ks, par = (uint32_t)j & 1u;
                 const bool more = j + 1 < nt;
-                if (!(ok = wait_for(kv_full + 8 * ks, kph, abort_flag, 43))) break;
+                if (!(ok = wait_one(kv_full + 8 * ks, kph, abort_flag, 43))) break;
                 next();
-                if (!(ok = wait_for(p_ready, par, abort_flag, 44))) break;
+                if (!(ok = wait_one(p_ready, par, abort_flag, 44))) break;
                 tc_fence_after();
                 output(0, vs, j > 0);
                 if (more) {
-                    if (!(ok = wait_for(kv_full + 8 * ks, kph, abort_flag, 43))) break;
+                    if (!(ok = wait_one(kv_full + 8 * ks, kph, abort_flag, 43))) break;
                     tc_fence_after();
                     scores(0, ks);
-                } else if (leader) tc_commit(o_full);
+                } else tc_commit(o_full);
                 if (two) {
-                    if (!(ok = wait_for(p_ready + 8, par, abort_flag, 44))) break;
+                    if (!(ok = wait_one(p_ready + 8, par, abort_flag, 44))) break;
                     tc_fence_after();
                     output(1, vs, j > 0);
                 }
-                if (leader) tc_commit(kv_empty + 8 * vs);
+                tc_commit(kv_empty + 8 * vs);
                 if (more) {
                     if (two) scores(1, ks);
-                    if (leader) tc_commit(kv_empty + 8 * ks);
+                    tc_commit(kv_empty + 8 * ks);
                     next();
-                } else if (two && leader) tc_commit(o_full + 8);
+                } else if (two) tc_commit(o_full + 8);
             }
         }
     } else {
@@ -327,7 +356,8 @@ __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_const
             }
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
             #pragma unroll
-            for (int k = 0; k < 128; ++k) mx[k & 3] = fmaxf(mx[k & 3], __uint_as_float(s[k]));
+            for (int k = 0; k < 128; k += 2)
+                asm("max.f32 %0, %0, %1, %2;" : "+f"(mx[(k >> 1) & 3]) : "f"(__uint_as_float(s[k])), "f"(__uint_as_float(s[k + 1])));
             const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
             const bool grow = (top - m) * c > GROWTH;        // (from -inf: any; -inf itself: NaN, false)
             if (__any_sync(0xFFFFFFFFu, grow)) {
@@ -358,13 +388,13 @@ __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_const
                 for (int k = 0; k < 16; ++k) {
                     float x, y;
                     fma2(x, y, __uint_as_float(s[32 * q + 2 * k]), __uint_as_float(s[32 * q + 2 * k + 1]), c, off);
-                    x = exp2_fast(x); y = exp2_fast(y);
-                    add2(sum[2 * (k & 1)], sum[2 * (k & 1) + 1], x, y);
+                    if ((k & 3) == 3) exp2_pair(x, y);          // a quarter of them
+                    else { x = exp2_fast(x); y = exp2_fast(y); }
                     w[k] = Word<E>::pack(x, y);
+                    s[32 * q + 2 * k] = __float_as_uint(x); s[32 * q + 2 * k + 1] = __float_as_uint(y);
                 }
                 tc_st16(s_col + 16 * q, w);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             if (!whole && t == 0) {
                 // infinities and NaNs among this tile's values: thread = key
                 if (!(ok = wait_for(kv_full + 8 * vs, vph, abort_flag, 46))) break;
@@ -398,6 +428,9 @@ __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_const
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(p_ready + 8 * t);
+            #pragma unroll
+            for (int k = 0; k < 64; ++k) add2(sum[2 * (k & 1)], sum[2 * (k & 1) + 1], __uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]));
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         }
         // ---- the rows' results ----
         if (ok && (t == 0 || two)) {
