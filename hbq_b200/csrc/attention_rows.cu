@@ -115,25 +115,23 @@ __global__ void __launch_bounds__(RW * 32) attention_rows_kernel(const __grid_co
         }
 
     auto load = [&](int64_t u, int stage) {
-        // a row of NK * 2 pieces of 16 bytes; two lanes share a key
-        const int key = lane >> 1;
-        const int64_t x = u + key;
-        const bool in = x < u1;
-        const E *kp = kb, *vp = vb;
-        if (in) {
-            if (x < a.P) { kp = pk + x * a.pks[1]; vp = pv + x * a.pvs[1]; }
-            else {
-                const int64_t y = x - a.P, j = y < ns ? y : lo + (y - ns);
-                kp = kb + j * a.ks[2]; vp = vb + j * a.vs[2];
-            }
-        }
-        const uint32_t dst = ring + stage * Sh::STAGE + key * Sh::ROW;
+        // a row of 2 NK pieces of 16 bytes, neighbouring lanes along a row: whole lines from memory
+        const uint32_t dst = ring + stage * Sh::STAGE;
         #pragma unroll
         for (int c = 0; c < NK; ++c) {
-            const int d = (2 * c + (lane & 1)) * 8;
-            const bool live = in && (uint32_t)d < a.D;
-            copy16(dst + d * 2, kp + (live ? d : 0), live);
-            copy16(dst + GROUP * Sh::ROW + d * 2, vp + (live ? d : 0), live);
+            const int x = lane + 32 * c, key = x / (2 * NK), d = (x - key * (2 * NK)) * 8;
+            const int64_t y = u + key;
+            const E *kp = kb, *vp = vb;
+            const bool live = y < u1 && (uint32_t)d < a.D;
+            if (live) {
+                if (y < a.P) { kp = pk + y * a.pks[1] + d; vp = pv + y * a.pvs[1] + d; }
+                else {
+                    const int64_t z = y - a.P, j = z < ns ? z : lo + (z - ns);
+                    kp = kb + j * a.ks[2] + d; vp = vb + j * a.vs[2] + d;
+                }
+            }
+            copy16(dst + key * Sh::ROW + d * 2, kp, live);
+            copy16(dst + (GROUP + key) * Sh::ROW + d * 2, vp, live);
         }
     };
 
