@@ -32,8 +32,12 @@ bool nothing(const hbq_attention* p) { return p->B == 0 || p->L == 0 || p->H == 
 // where its rows (of all sequences) are more than the warp-level MMA's 16.
 struct Plan {
     bool own_tc, prefix_tc;            // prefix_tc: the prefix has a launch of its own, else it is part of the rows' list
-    int own, prefix;                   // pieces
-    int parts() const { return own + prefix; }
+    int prefix, own;                   // the tensor-core kernel's pieces
+    int blocks, shared;                // the few-row kernel's blocks (0: not launched)
+    int parts;                         // entries of a row's list of parts; 0: every row is written by one block
+    int64_t part_bytes, table_bytes, slot_bytes;
+    int64_t bytes() const { return part_bytes + table_bytes + slot_bytes; }
+    bool join() const { return parts > 0 || shared; }
 };
 Plan plan_of(const hbq_attention* p)
 {
@@ -42,17 +46,24 @@ Plan plan_of(const hbq_attention* p)
     const bool alone = p->P == 0 || c.prefix_tc;
     c.own_tc = alone && p->L > 1 && p->S > 0;
     if (c.prefix_tc) c.prefix = attention_tc_parts(p, true);
-    if (!c.prefix_tc || p->S > 0) c.own = c.own_tc ? attention_tc_parts(p, false) : attention_rows_parts(p, !alone);
+    if (c.own_tc) c.own = attention_tc_parts(p, false);
+    else if (!c.prefix_tc || p->S > 0) c.blocks = attention_rows_blocks(p, !alone, &c.shared);
+    c.parts = c.prefix + c.own + (c.prefix_tc && c.blocks ? 1 : 0);
+    if (c.parts == 1) c.parts = 0;
+    const auto up = [](int64_t n) { return (n + 15) / 16 * 16; };
+    c.part_bytes = up(p->B * p->L * p->H * c.parts * (p->D + 2) * 4);
+    if (c.shared) {
+        c.table_bytes = up((p->B * p->L + 1) * 8);
+        c.slot_bytes = up((int64_t)c.blocks * 2 * 16 * (p->D + 2) * 4);
+    }
     return c;
 }
-
-int64_t part_bytes(const hbq_attention* p, int64_t parts) { return parts > 1 ? p->B * p->L * p->H * parts * (p->D + 2) * 4 : 0; }
 
 }  // namespace
 
 int64_t attention_workspace_bytes(const hbq_attention* p)
 {
-    return check(p) || nothing(p) ? 0 : part_bytes(p, plan_of(p).parts());
+    return check(p) || nothing(p) ? 0 : plan_of(p).bytes();
 }
 
 int attention_run(const hbq_attention* p, void* workspace, int64_t workspace_bytes, cudaStream_t stream)
@@ -67,22 +78,29 @@ int attention_run(const hbq_attention* p, void* workspace, int64_t workspace_byt
     a.B = (uint32_t)p->B; a.L = (uint32_t)p->L; a.H = (uint32_t)p->H; a.Hkv = (uint32_t)p->Hkv; a.G = (uint32_t)(p->H / p->Hkv); a.D = (uint32_t)p->D;
     a.scale_log2 = p->scale * 1.4426950408889634f;
     const Plan c = plan_of(p);
-    a.parts = c.parts();
-    const int64_t need = part_bytes(p, a.parts);
+    if (c.blocks < 0) return HBQ_ERR_UNSUPPORTED;
+    const int64_t need = c.bytes();
     if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))) return HBQ_ERR_WORKSPACE;
-    a.part = static_cast<float*>(workspace);
+    a.parts = c.parts; a.blocks = c.blocks; a.shared = c.shared;
+    char* ws = static_cast<char*>(workspace);
+    a.part = reinterpret_cast<float*>(ws);
+    a.table = reinterpret_cast<int64_t*>(ws + c.part_bytes);
+    a.slots = reinterpret_cast<float*>(ws + c.part_bytes + c.table_bytes);
     if (c.prefix_tc) {
         a.nsplit = c.prefix;
         { const int rc = attention_tc_launch(a, p->dtype, true, stream); if (rc) return rc; }
         a.P = 0;
         a.part0 = c.prefix;
     }
-    if (c.own) {
+    if (c.own_tc) {
         a.nsplit = c.own;
-        const int rc = c.own_tc ? attention_tc_launch(a, p->dtype, false, stream) : attention_rows_launch(a, p->dtype, stream);
+        const int rc = attention_tc_launch(a, p->dtype, false, stream);
+        if (rc) return rc;
+    } else if (c.blocks) {
+        const int rc = attention_rows_launch(a, p->dtype, stream);
         if (rc) return rc;
     }
-    return a.parts > 1 ? attention_join_launch(a, p->dtype, stream) : HBQ_OK;
+    return c.join() ? attention_join_launch(a, p->dtype, stream) : HBQ_OK;
 }
 
 }  // namespace hbq

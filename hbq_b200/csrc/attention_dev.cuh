@@ -12,9 +12,13 @@ struct AttnArgs {
     int64_t S, P, window, sinks;
     uint32_t B, L, H, Hkv, G, D;
     float scale_log2;                                        // scale * log2(e)
-    int nsplit;
+    int nsplit;                                              // (tensor-core kernel) pieces of a block's keys
     float* part;                                             // [rows][parts][D] sums, then [rows][parts] (maximum, weight)
     int parts, part0;
+    // The few-row kernel's division of work: `blocks` blocks of equal shares; its table and slots in the workspace.
+    int blocks, shared;                                      // shared: shares may begin and end inside a row group
+    int64_t* table;                                          // [B * L + 1] units before each token
+    float* slots;                                            // [blocks][2][16][D] sums, then [blocks][2][16] (maximum, weight)
 };
 
 // Rows of sequence b: its keys, and the position of its first row.
@@ -40,10 +44,25 @@ __device__ __forceinline__ float2* part_weight(const AttnArgs& a, int64_t row, i
     return reinterpret_cast<float2*>(a.part + (int64_t)a.B * a.L * a.H * a.parts * a.D) + row * a.parts + part;
 }
 
-int attention_join_launch(const AttnArgs& a, int dtype, cudaStream_t stream);                    // attention_rows.cu
-int attention_rows_launch(AttnArgs& a, int dtype, cudaStream_t stream);
-int attention_rows_parts(const hbq_attention* p, bool prefix);
-int attention_tc_launch(AttnArgs& a, int dtype, bool prefix, cudaStream_t stream);               // attention_tc.cu
+// The few-row kernel's units of work: 64 keys of one row group (16 heads of a key head, one token).  A token's groups all
+// have the same number of units.
+constexpr int ROWS_UNIT = 64;
+// Block c of n has units total * c / n up to total * (c + 1) / n; no more blocks take part than there are units, so that each
+// has some and a group's blocks follow one another.
+__device__ __forceinline__ int64_t rows_takers(const AttnArgs& a, int64_t total) { return total < a.blocks ? total : a.blocks; }
+__device__ __forceinline__ int rows_owner(int64_t unit, int64_t total, int64_t takers) { return (int)(((unit + 1) * takers - 1) / total); }
+__device__ __forceinline__ float* slot_sum(const AttnArgs& a, int block, int which, int row) { return a.slots + ((int64_t)(block * 2 + which) * 16 + row) * a.D; }
+__device__ __forceinline__ float2* slot_weight(const AttnArgs& a, int block, int which, int row)
+{
+    return reinterpret_cast<float2*>(a.slots + (int64_t)a.blocks * 2 * 16 * a.D) + (block * 2 + which) * 16 + row;
+}
+
+// attention_rows.cu
+int attention_rows_launch(const AttnArgs& a, int dtype, cudaStream_t stream);
+int attention_join_launch(const AttnArgs& a, int dtype, cudaStream_t stream);
+int attention_rows_blocks(const hbq_attention* p, bool prefix, int* shared);
+// attention_tc.cu
+int attention_tc_launch(AttnArgs& a, int dtype, bool prefix, cudaStream_t stream);
 int attention_tc_parts(const hbq_attention* p, bool prefix);
 
 }  // namespace hbq

@@ -6,8 +6,11 @@
 // heads; one MMA tile is 16 rows by 8 keys, most of them empty for four heads, at a cost far below the memory's.
 //
 // Each warp has a ring of its own (16 keys and values a stage, asynchronous copies), a maximum, a weight and a sum of its
-// own; no barrier until the warps' sums are joined at the end.  With few sequences the list is cut over several blocks,
-// whose parts (sum, maximum, weight) a second kernel joins.
+// own; no barrier until the warps' sums are joined at the end of a row group.
+//
+// The lengths are known on the device alone and may be as different as one key and a hundred thousand.  So the groups'
+// units of 64 keys form one list over all sequences, of which every block (two an SM) takes an equal share; where a share
+// begins or ends inside a group, its part (sum, maximum, weight) goes to a slot of the block and a second kernel joins.
 #include "attention_dev.cuh"
 
 namespace hbq {
@@ -66,36 +69,98 @@ template <int NK> struct RowsShape {
     static constexpr int BYTES = RING > JOIN ? RING : JOIN;
 };
 
+// The keys of row (b, i): U entries -- the prefix, `ns` first keys, then those from lo on.
+struct KeyList { int64_t U, lo, ns; };
+__device__ __forceinline__ KeyList keys_of(const AttnArgs& a, uint32_t b, uint32_t i)
+{
+    int64_t n, p;
+    sequence_of(a, b, &n, &p);
+    p += i;
+    KeyList k = {0, 0, 0};
+    if (p < n) {
+        k.U = a.P;
+        if (p >= 0) {
+            k.lo = a.window > 0 && p - a.window + 1 > 0 ? p - a.window + 1 : 0;
+            k.ns = a.sinks < k.lo ? a.sinks : k.lo;
+            k.U += k.ns + (p + 1 - k.lo);
+        }
+    }
+    return k;
+}
+// A group's units; one that sees nothing has one, in which its zeros are written.
+__device__ __forceinline__ int64_t units_of(const KeyList& k) { return k.U > ROWS_UNIT ? (k.U + ROWS_UNIT - 1) / ROWS_UNIT : 1; }
+
+// Units before each token, [0 .. tokens], by the whole block (tokens at most two a thread).
+__device__ void count_units(const AttnArgs& a, int64_t* table)
+{
+    __shared__ int64_t warps[RW];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t tokens = a.B * a.L, r = 2 * threadIdx.x;
+    int64_t c0 = 0, c1 = 0;
+    if (r < tokens) c0 = units_of(keys_of(a, r / a.L, r % a.L));
+    if (r + 1 < tokens) c1 = units_of(keys_of(a, (r + 1) / a.L, (r + 1) % a.L));
+    int64_t sum = c0 + c1;
+    #pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const int64_t below = __shfl_up_sync(0xFFFFFFFFu, sum, d);
+        if (lane >= d) sum += below;
+    }
+    if (lane == 31) warps[warp] = sum;
+    __syncthreads();
+    int64_t before = sum - c0 - c1;
+    for (int w = 0; w < warp; ++w) before += warps[w];
+    if (r < tokens) { table[r] = before; table[r + 1] = before + c0; }
+    if (r + 1 < tokens) table[r + 2] = before + c0 + c1;
+    __syncthreads();
+}
+
 template <class E, int NK>
 __global__ void __launch_bounds__(RW * 32) attention_rows_kernel(const __grid_constant__ AttnArgs a, uint32_t tiles)
 {
     using Sh = RowsShape<NK>;
     extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ int64_t table[RW * 64 + 1];
     grid_dependency_wait();
     dependents_may_start();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    uint32_t id = blockIdx.x;
-    const uint32_t split = id % (uint32_t)a.nsplit; id /= (uint32_t)a.nsplit;
-    const uint32_t tile = id % tiles; id /= tiles;
-    const uint32_t hk = id % a.Hkv; id /= a.Hkv;
-    const uint32_t i = id % a.L, b = id / a.L;
-    const uint32_t g0 = tile * 16, rows = min(16u, a.G - g0), h0 = hk * a.G + g0;
-
-    // the list of visible keys, and this block's piece of it
-    int64_t n, p;
-    sequence_of(a, b, &n, &p);
-    p += i;
-    int64_t lo = 0, ns = 0, U = 0;
-    if (p < n) {
-        U = a.P;
-        if (p >= 0) {
-            lo = a.window > 0 && p - a.window + 1 > 0 ? p - a.window + 1 : 0;
-            ns = a.sinks < lo ? a.sinks : lo;
-            U += ns + (p + 1 - lo);
+    const uint32_t groups = a.Hkv * tiles, tokens = a.B * a.L;       // row groups of a token
+    int64_t w0, w1;                                                  // this block's share of the units
+    uint32_t token;
+    if (a.shared) {
+        count_units(a, table);
+        if (blockIdx.x == 0)
+            for (uint32_t r = threadIdx.x; r <= tokens; r += RW * 32) a.table[r] = table[r];
+        const int64_t total = table[tokens] * groups;
+        const int64_t takers = rows_takers(a, total);
+        if (blockIdx.x >= takers) return;
+        w0 = total * blockIdx.x / takers; w1 = total * (blockIdx.x + 1) / takers;
+        uint32_t low = 0, high = tokens;                             // the last token that begins at or before w0
+        while (high - low > 1) {
+            const uint32_t mid = (low + high) / 2;
+            if (table[mid] * groups <= w0) low = mid; else high = mid;
         }
+        token = low;
+    } else {
+        token = blockIdx.x / groups;
+        w0 = 0; w1 = 1;
     }
-    const int64_t piece = ((U + a.nsplit - 1) / a.nsplit + RW * GROUP - 1) / (RW * GROUP) * (RW * GROUP);
-    const int64_t u0 = (int64_t)split * piece, u1 = U < u0 + piece ? U : u0 + piece;
+    while (w0 < w1) {
+    const uint32_t b = token / a.L, i = token - b * a.L;
+    const KeyList list = keys_of(a, b, i);
+    const int64_t lo = list.lo, ns = list.ns, U = list.U;
+    int64_t u0 = 0, u1 = U, take = 1;
+    uint32_t g;
+    int slot = -1;                                                   // -1: the whole group
+    if (a.shared) {
+        const int64_t units = table[token + 1] - table[token], in = w0 - table[token] * groups;
+        g = (uint32_t)(in / units);
+        const int64_t off = in - g * units;
+        take = min(units - off, w1 - w0);
+        u0 = off * ROWS_UNIT;
+        if ((off + take) * ROWS_UNIT < U) u1 = (off + take) * ROWS_UNIT;
+        slot = take == units ? -1 : off > 0 ? 0 : 1;
+    } else g = blockIdx.x - token * groups;
+    const uint32_t hk = g / tiles, g0 = (g - hk * tiles) * 16, rows = min(16u, a.G - g0), h0 = hk * a.G + g0;
 
     const E* kb = static_cast<const E*>(a.k) + (int64_t)b * a.ks[0] + (int64_t)hk * a.ks[1];
     const E* vb = static_cast<const E*>(a.v) + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[1];
@@ -242,57 +307,95 @@ __global__ void __launch_bounds__(RW * 32) attention_rows_kernel(const __grid_co
             sum = fmaf(js[(w * 16 + row) * Sh::DP + d], f, sum);
             weight = fmaf(jm[(w * 16 + row) * 2 + 1], f, weight);
         }
-        if (a.parts > 1) {
+        if (slot >= 0) {
+            slot_sum(a, blockIdx.x, slot, row)[d] = sum;
+            if (d == 0) *slot_weight(a, blockIdx.x, slot, row) = make_float2(top, weight);
+        } else if (a.parts > 0) {
             const int64_t at = ((int64_t)b * a.L + i) * a.H + h0 + row;
-            part_sum(a, at, a.part0 + split)[d] = sum;
-            if (d == 0) *part_weight(a, at, a.part0 + split) = make_float2(top, weight);
+            part_sum(a, at, a.part0)[d] = sum;
+            if (d == 0) *part_weight(a, at, a.part0) = make_float2(top, weight);
         } else {
             Mma<E>::store(a.out, (int64_t)b * a.os[0] + (int64_t)i * a.os[1] + (int64_t)(h0 + row) * a.os[2] + d, weight == 0.f ? 0.f : sum / weight);
         }
     }
+    w0 += take;
+    if (a.shared && w0 < w1) {
+        if (w0 >= table[token + 1] * groups) ++token;
+        __syncthreads();                                             // the join's memory becomes the ring again
+    }
+    }
 }
 
-// One warp joins a row's parts: maxima, then weights and sums relative to the largest.
+// One warp joins a row's parts: the tensor-core kernel's, and the few-row kernel's part or slots.  Maxima, then weights and
+// sums relative to the largest.
 template <class E>
-__global__ void __launch_bounds__(256) attention_join_kernel(const __grid_constant__ AttnArgs a)
+__global__ void __launch_bounds__(64) attention_join_kernel(const __grid_constant__ AttnArgs a, uint32_t tiles)
 {
     grid_dependency_wait();
     dependents_may_start();
     const int lane = threadIdx.x & 31;
-    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int64_t row = (int64_t)blockIdx.x * 2 + (threadIdx.x >> 5);
     if (row >= (int64_t)a.B * a.L * a.H) return;
-    const float2* w = part_weight(a, row, 0);
+    const int64_t token = row / a.H;
+    const uint32_t h = (uint32_t)(row - token * a.H);
+    int first = 0, count = a.parts, listed = a.parts, gr = 0;       // parts 0 .. listed - 1 lie in the row's list, the rest in slots
+    if (a.shared) {
+        const uint32_t hk = h / a.G, gg = h - hk * a.G, groups = a.Hkv * tiles;
+        gr = (int)(gg & 15);
+        const int64_t* table = behind_wait(a.table);
+        const int64_t begin = table[token], units = table[token + 1] - begin, total = table[(int64_t)a.B * a.L] * groups;
+        const int64_t s0 = begin * groups + (int64_t)(hk * tiles + gg / 16) * units;
+        const int64_t takers = rows_takers(a, total);
+        first = rows_owner(s0, total, takers);
+        const int last = rows_owner(s0 + units - 1, total, takers);
+        if (first < last) {
+            if (listed > 0) --listed;                                // (the entry for an undivided group is not in use)
+            count = listed + last - first + 1;
+        } else if (a.parts == 0) return;                             // undivided: written already
+    }
+    const auto weight_of = [&](int s) { return s < listed ? *part_weight(a, row, s) : *slot_weight(a, first + s - listed, s == listed, gr); };
+    const auto sum_of = [&](int s) { return (s < listed ? part_sum(a, row, s) : slot_sum(a, first + s - listed, s == listed, gr)); };
     float top = -INFINITY;
-    for (int s = lane; s < a.parts; s += 32) top = fmaxf(top, w[s].x);
+    for (int s = lane; s < count; s += 32) {
+        const float2 ml = weight_of(s);
+        if (ml.y != 0.f) top = fmaxf(top, ml.x);
+    }
     #pragma unroll
     for (int k = 16; k; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, k));
     const float ref = top == -INFINITY ? 0.f : top;
     float weight = 0.f, sum[4] = {};
-    for (int s = 0; s < a.parts; ++s) {
-        const float2 ml = w[s];
-        if (ml.y == 0.f) continue;                       // an empty part's sums are not looked at
-        const float f = exp2_fast(ml.x - ref);
-        weight = fmaf(ml.y, f, weight);
-        const float* x = part_sum(a, row, s);
+    const bool in = lane * 4 < (int)a.D;
+    for (int s0 = 0; s0 < count; s0 += 32) {
+        float f = 0.f;
+        if (s0 + lane < count) {
+            const float2 ml = weight_of(s0 + lane);
+            if (ml.y != 0.f) { f = exp2_fast(ml.x - ref); weight = fmaf(ml.y, f, weight); }
+        }
+        const int end = min(32, count - s0);
+        #pragma unroll 4
+        for (int s = 0; s < end; ++s) {
+            const float g = __shfl_sync(0xFFFFFFFFu, f, s);
+            if (g != 0.f && in) {                                    // an empty part's sums are not looked at (a NaN is no zero)
+                const float4 x = *reinterpret_cast<const float4*>(sum_of(s0 + s) + lane * 4);
+                sum[0] = fmaf(x.x, g, sum[0]); sum[1] = fmaf(x.y, g, sum[1]); sum[2] = fmaf(x.z, g, sum[2]); sum[3] = fmaf(x.w, g, sum[3]);
+            }
+        }
+    }
+    #pragma unroll
+    for (int k = 16; k; k >>= 1) weight += __shfl_xor_sync(0xFFFFFFFFu, weight, k);
+    const int64_t b = token / a.L, i = token - b * a.L;
+    if (in) {
         #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (lane + 32 * e < (int)a.D) sum[e] = fmaf(x[lane + 32 * e], f, sum[e]);
+            Mma<E>::store(a.out, b * a.os[0] + i * a.os[1] + h * a.os[2] + lane * 4 + e, weight == 0.f ? 0.f : sum[e] / weight);
     }
-    const int64_t h = row % a.H, bl = row / a.H, i = bl % a.L, b = bl / a.L;
-    #pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (lane + 32 * e < (int)a.D)
-            Mma<E>::store(a.out, b * a.os[0] + i * a.os[1] + h * a.os[2] + lane + 32 * e, weight == 0.f ? 0.f : sum[e] / weight);
 }
 
 template <class E, int NK>
 int rows_launch(const AttnArgs& a, cudaStream_t stream)
 {
-    const uint32_t tiles = (a.G + 15) / 16;
-    const int64_t blocks = (int64_t)a.B * a.L * a.Hkv * tiles * a.nsplit;
-    if (blocks > 0x7FFFFFFFll) return HBQ_ERR_UNSUPPORTED;
     { const int rc = ensure_dynamic_smem(attention_rows_kernel<E, NK>, RowsShape<NK>::BYTES); if (rc) return rc; }
-    HBQ_CUDA_TRY(launch_dependent(attention_rows_kernel<E, NK>, (unsigned)blocks, RW * 32, (size_t)RowsShape<NK>::BYTES, stream, a, tiles));
+    HBQ_CUDA_TRY(launch_dependent(attention_rows_kernel<E, NK>, (unsigned)a.blocks, RW * 32, (size_t)RowsShape<NK>::BYTES, stream, a, (a.G + 15) / 16));
     HBQ_LAUNCH_CHECK("attention_rows_kernel");
     return HBQ_OK;
 }
@@ -311,33 +414,38 @@ int rows_type(const AttnArgs& a, cudaStream_t stream)
 
 }  // namespace
 
-// Into how many pieces a row's list of keys is cut; prefix: the list begins with it.
-int attention_rows_parts(const hbq_attention* p, bool prefix)
+// Blocks of the few-row kernel; prefix: a row's list begins with it.  Shares of equal size over two blocks an SM; a block a
+// row group where there are too many tokens for the table, or where every group is a unit or two by its bounds alone.
+int attention_rows_blocks(const hbq_attention* p, bool prefix, int* shared)
 {
     int sms = 148;
     device_sms(&sms);
-    const int64_t blocks = p->B * p->L * p->Hkv * ((p->H / p->Hkv + 15) / 16);
+    const int64_t groups = p->Hkv * ((p->H / p->Hkv + 15) / 16), tokens = p->B * p->L;
     int64_t keys = p->S;
     if (p->window > 0 && p->window + p->sinks < keys) keys = p->window + p->sinks;
     if (prefix) keys += p->P;
-    // two blocks an SM are resident; twice as many pieces as that even out sequences of different lengths, as far as a
-    // piece keeps 128 keys
-    int64_t n = ((int64_t)sms * 4 + blocks - 1) / blocks;
-    if (n > (keys + 127) / 128) n = (keys + 127) / 128;
-    return (int)(n < 1 ? 1 : n > 256 ? 256 : n);
+    const int64_t units = (keys + ROWS_UNIT - 1) / ROWS_UNIT;
+    if (tokens > RW * 64 || units <= 1) {
+        *shared = 0;
+        return groups * tokens > 0x7FFFFFFF ? -1 : (int)(groups * tokens);
+    }
+    *shared = 1;
+    const int64_t most = units * groups * tokens;
+    return (int)(most < 2 * sms ? most : 2 * sms);
 }
 
-int attention_rows_launch(AttnArgs& a, int dtype, cudaStream_t stream)
+int attention_rows_launch(const AttnArgs& a, int dtype, cudaStream_t stream)
 {
     return dtype == HBQ_DTYPE_F16 ? rows_type<__half>(a, stream) : rows_type<__nv_bfloat16>(a, stream);
 }
 
 int attention_join_launch(const AttnArgs& a, int dtype, cudaStream_t stream)
 {
-    const int64_t blocks = ((int64_t)a.B * a.L * a.H + 7) / 8;
+    const int64_t blocks = ((int64_t)a.B * a.L * a.H + 1) / 2;
     if (blocks > 0x7FFFFFFFll) return HBQ_ERR_UNSUPPORTED;
-    if (dtype == HBQ_DTYPE_F16) HBQ_CUDA_TRY(launch_dependent(attention_join_kernel<__half>, (unsigned)blocks, 256, 0, stream, a));
-    else HBQ_CUDA_TRY(launch_dependent(attention_join_kernel<__nv_bfloat16>, (unsigned)blocks, 256, 0, stream, a));
+    const uint32_t tiles = (a.G + 15) / 16;
+    if (dtype == HBQ_DTYPE_F16) HBQ_CUDA_TRY(launch_dependent(attention_join_kernel<__half>, (unsigned)blocks, 64, 0, stream, a, tiles));
+    else HBQ_CUDA_TRY(launch_dependent(attention_join_kernel<__nv_bfloat16>, (unsigned)blocks, 64, 0, stream, a, tiles));
     HBQ_LAUNCH_CHECK("attention_join_kernel");
     return HBQ_OK;
 }

@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_const
         if (ok && (t == 0 || two)) {
             if (nt > 0) ok = wait_for(o_full + 8 * t, 0, abort_flag, 47);
             tc_fence_after();
-            const bool direct = a.parts == 1, add = nt > 0 && *special;
+            const bool direct = a.parts == 0, add = nt > 0 && *special;
             const bool live = hi >= 0 && l != 0.f;            // (a NaN counts as something)
             const float f = direct ? (live ? 1.f / l : 0.f) : 1.f;
             const int64_t row = ((int64_t)b * a.L + i) * a.H + h;
