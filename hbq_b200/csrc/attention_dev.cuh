@@ -1,6 +1,7 @@
 // What the attention kernels share: which keys a row sees, and the form in which parts of a row's sum are joined.
 #pragma once
 #include "common.cuh"
+#include <cuda.h>
 
 namespace hbq {
 
@@ -46,7 +47,6 @@ __device__ __forceinline__ float2* part_weight(const AttnArgs& a, int64_t row, i
 
 // The few-row kernel's units of work: 64 keys of one row group (16 heads of a key head, one token).  A token's groups all
 // have the same number of units.
-constexpr int ROWS_UNIT = 64;
 // Block c of n has units total * c / n up to total * (c + 1) / n; no more blocks take part than there are units, so that each
 // has some and a group's blocks follow one another.
 __device__ __forceinline__ int64_t rows_takers(const AttnArgs& a, int64_t total) { return total < a.blocks ? total : a.blocks; }
@@ -64,5 +64,7 @@ int attention_rows_blocks(const hbq_attention* p, bool prefix, int* shared);
 // attention_tc.cu
 int attention_tc_launch(AttnArgs& a, int dtype, bool prefix, cudaStream_t stream);
 int attention_tc_parts(const hbq_attention* p, bool prefix);
+int attention_cache_map(CUtensorMap* map, const void* ptr, int dtype, int64_t D, int rows, int64_t keys, int64_t key_stride, int64_t heads,
+                        int64_t head_stride, int64_t seqs, int64_t seq_stride);
 
 }  // namespace hbq

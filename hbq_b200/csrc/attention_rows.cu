@@ -1,23 +1,33 @@
 // Attention of few rows against a cache: the query heads that share a key head, for one token, on the warp-level MMA.
 //
-// For a row at position p the visible keys are the prefix, the first `sinks` ones and those behind p - window: a list
-// u = 0 .. U - 1 whose entries map to rows of the cache.  Every lane loads list entries, so nothing that the mask hides is
-// read at all, and entries behind the list's end are zeros.  Bound by memory: keys and values are read once for up to 16
-// heads; one MMA tile is 16 rows by 8 keys, most of them empty for four heads, at a cost far below the memory's.
+// For a row at position p the visible keys are the prefix, the first `sinks` ones and those behind p - window: three runs of
+// the cache, walked over in steps of 16 keys.  Nothing that the mask hides enters the arithmetic: a run's last step may
+// bring keys behind its end, whose scores become -inf and whose values zeros.  Bound by memory: keys and values are read once
+// for up to 16 heads; one MMA tile is 16 rows by 8 keys, most of them empty for four heads, at a cost below the memory's.
 //
-// Each warp has a ring of its own (16 keys and values a stage, asynchronous copies), a maximum, a weight and a sum of its
-// own; no barrier until the warps' sums are joined at the end of a row group.
+// Each warp has a ring of its own, filled by TMA (one lane; with asynchronous copies by all lanes the addresses took most of
+// the instructions, and the kernel was bound by their latency at 4.7 TB/s), a maximum, a weight and a sum of its own; no
+// barrier until the warps' sums are joined at the end of a row group.  As in the tensor-core kernel the sums are rescaled only
+// when a maximum has grown by more than 2^8 in the weights, so a step without that has no exchange between lanes.
 //
-// The lengths are known on the device alone and may be as different as one key and a hundred thousand.  So the groups'
-// units of 64 keys form one list over all sequences, of which every block (two an SM) takes an equal share; where a share
+// The lengths are known on the device alone and may be as different as one key and a hundred thousand.  So the row groups'
+// units of 64 keys form one list over all sequences, of which every block takes an equal share; where a share
 // begins or ends inside a group, its part (sum, maximum, weight) goes to a slot of the block and a second kernel joins.
 #include "attention_dev.cuh"
+#include "tc_dev.cuh"
 
+#ifndef ROWS_STAGES
+#define ROWS_STAGES 3
+#define ROWS_CTAS 2
+#endif
 namespace hbq {
 
 namespace {
 
-constexpr int RW = 4, STAGES = 3, GROUP = 16;      // warps, stages a warp, keys a stage
+constexpr int RW = 4, STAGES = ROWS_STAGES, GROUP = 16;      // warps, stages a warp, keys a stage
+constexpr int BLOCKS_PER_SM = ROWS_CTAS;
+constexpr uint32_t POLLS = 1u << 20;
+constexpr float SHIFT = 4.f, GROWTH = 8.f;          // as in the tensor-core kernel
 
 template <class E> struct Mma;
 template <> struct Mma<__half> {
@@ -45,11 +55,6 @@ template <> struct Mma<__nv_bfloat16> {
     static __device__ __forceinline__ void store(void* p, int64_t i, float v) { static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v); }
 };
 
-__device__ __forceinline__ uint32_t smem_of(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool live)
-{
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
-}
 __device__ __forceinline__ void ldsm4(uint32_t* r, uint32_t addr)
 {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -61,34 +66,48 @@ __device__ __forceinline__ void ldsm4t(uint32_t* r, uint32_t addr)
 
 template <int NK> struct RowsShape {
     static constexpr int DP = NK * 16;                       // head length, rounded up
-    static constexpr int ROW = DP * 2 + 16;                  // bytes of a staged row: an odd number of 16-byte pieces, so that
-                                                             // the eight rows of an 8 x 8 matrix lie in different banks
-    static constexpr int STAGE = 2 * GROUP * ROW;
+    static constexpr int HALVES = (DP + 63) / 64, TILE = HALVES * GROUP * 128;       // 128-byte rows, swizzled by TMA
+    static constexpr int STAGE = 2 * TILE;
     static constexpr int RING = RW * STAGES * STAGE;
     static constexpr int JOIN = RW * 16 * (DP + 2) * 4;
     static constexpr int BYTES = RING > JOIN ? RING : JOIN;
 };
 
-// The keys of row (b, i): U entries -- the prefix, `ns` first keys, then those from lo on.
-struct KeyList { int64_t U, lo, ns; };
+// The maps of a call's cache and prefix.
+struct RowsMaps { CUtensorMap k, v, pk, pv; };
+
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar) : "memory");
+}
+
+// The keys of row (b, i) in steps of 16: the prefix's, those of the first `ns` keys, those of keys lo .. p.
+struct KeyList {
+    int P, ns, lo, end;                                      // lengths of the first two runs; the third is lo .. end - 1
+    int pre, sink, steps;                                    // steps of the first run, the first two, and all
+};
 __device__ __forceinline__ KeyList keys_of(const AttnArgs& a, uint32_t b, uint32_t i)
 {
     int64_t n, p;
     sequence_of(a, b, &n, &p);
     p += i;
-    KeyList k = {0, 0, 0};
+    KeyList k = {};
     if (p < n) {
-        k.U = a.P;
+        k.P = (int)a.P;
         if (p >= 0) {
-            k.lo = a.window > 0 && p - a.window + 1 > 0 ? p - a.window + 1 : 0;
-            k.ns = a.sinks < k.lo ? a.sinks : k.lo;
-            k.U += k.ns + (p + 1 - k.lo);
+            k.lo = a.window > 0 && p - a.window + 1 > 0 ? (int)(p - a.window + 1) : 0;
+            k.ns = a.sinks < k.lo ? (int)a.sinks : k.lo;
+            k.end = (int)p + 1;
         }
     }
+    k.pre = k.P / GROUP + (k.P % GROUP != 0);
+    k.sink = k.pre + k.ns / GROUP + (k.ns % GROUP != 0);
+    k.steps = k.sink + (k.end - k.lo) / GROUP + ((k.end - k.lo) % GROUP != 0);
     return k;
 }
 // A group's units; one that sees nothing has one, in which its zeros are written.
-__device__ __forceinline__ int64_t units_of(const KeyList& k) { return k.U > ROWS_UNIT ? (k.U + ROWS_UNIT - 1) / ROWS_UNIT : 1; }
+__device__ __forceinline__ int64_t units_of(const KeyList& k) { return k.steps > RW ? (k.steps + RW - 1) / RW : 1; }
 
 // Units before each token, [0 .. tokens], by the whole block (tokens at most two a thread).
 __device__ void count_units(const AttnArgs& a, int64_t* table)
@@ -115,14 +134,24 @@ __device__ void count_units(const AttnArgs& a, int64_t* table)
 }
 
 template <class E, int NK>
-__global__ void __launch_bounds__(RW * 32) attention_rows_kernel(const __grid_constant__ AttnArgs a, uint32_t tiles)
+__global__ void __launch_bounds__(RW * 32, BLOCKS_PER_SM) attention_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ RowsMaps maps, uint32_t tiles)
 {
     using Sh = RowsShape<NK>;
-    extern __shared__ __align__(16) uint8_t smem[];
+    extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ int64_t table[RW * 64 + 1];
+    __shared__ __align__(8) uint64_t full[RW * STAGES];
+    __shared__ int given_up;
+    volatile int* abort_flag = &given_up;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int k = 0; k < RW * STAGES; ++k) mbar_init(smem_u32(&full[k]), 1);
+        given_up = (smem_u32(smem) & 1023u) != 0;                    // (the copies' swizzle goes by address bits)
+        if (given_up) atomicCAS(&g_tc_status, 0, 50);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
     grid_dependency_wait();
     dependents_may_start();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t groups = a.Hkv * tiles, tokens = a.B * a.L;       // row groups of a token
     int64_t w0, w1;                                                  // this block's share of the units
     uint32_t token;
@@ -144,11 +173,14 @@ __global__ void __launch_bounds__(RW * 32) attention_rows_kernel(const __grid_co
         token = blockIdx.x / groups;
         w0 = 0; w1 = 1;
     }
+    const uint32_t ring = smem_u32(smem) + warp * (STAGES * Sh::STAGE), bars = smem_u32(&full[warp * STAGES]);
+    uint32_t stage = 0, phase = 0;                                   // the warp's next stage to read, and its parity
+    bool ok = given_up == 0;
     while (w0 < w1) {
     const uint32_t b = token / a.L, i = token - b * a.L;
     const KeyList list = keys_of(a, b, i);
-    const int64_t lo = list.lo, ns = list.ns, U = list.U;
-    int64_t u0 = 0, u1 = U, take = 1;
+    int64_t take = 1;
+    int x0 = 0, x1 = list.steps;                                     // this share's steps of the group
     uint32_t g;
     int slot = -1;                                                   // -1: the whole group
     if (a.shared) {
@@ -156,17 +188,34 @@ __global__ void __launch_bounds__(RW * 32) attention_rows_kernel(const __grid_co
         g = (uint32_t)(in / units);
         const int64_t off = in - g * units;
         take = min(units - off, w1 - w0);
-        u0 = off * ROWS_UNIT;
-        if ((off + take) * ROWS_UNIT < U) u1 = (off + take) * ROWS_UNIT;
+        x0 = (int)off * RW;
+        x1 = (int)min((int64_t)list.steps, (off + take) * RW);
         slot = take == units ? -1 : off > 0 ? 0 : 1;
     } else g = blockIdx.x - token * groups;
     const uint32_t hk = g / tiles, g0 = (g - hk * tiles) * 16, rows = min(16u, a.G - g0), h0 = hk * a.G + g0;
+    const int kh = a.ks[1] > 0 ? (int)hk : 0, kb = a.ks[0] > 0 ? (int)b : 0, vh = a.vs[1] > 0 ? (int)hk : 0, vb = a.vs[0] > 0 ? (int)b : 0;
+    const int ph = a.pks[0] > 0 ? (int)hk : 0, pvh = a.pvs[0] > 0 ? (int)hk : 0;
 
-    const E* kb = static_cast<const E*>(a.k) + (int64_t)b * a.ks[0] + (int64_t)hk * a.ks[1];
-    const E* vb = static_cast<const E*>(a.v) + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[1];
-    const E* pk = static_cast<const E*>(a.pk) + (int64_t)hk * a.pks[0];
-    const E* pv = static_cast<const E*>(a.pv) + (int64_t)hk * a.pvs[0];
-    const uint32_t ring = smem_of(smem) + warp * (STAGES * Sh::STAGE);
+    // one lane: step x into a stage
+    auto load = [&](int x, uint32_t st) {
+        const uint32_t dst = ring + st * Sh::STAGE, bar = bars + 8 * st;
+        mbar_expect_tx(bar, Sh::STAGE);
+        const bool pre = x < list.pre;
+        const int j = pre ? x * GROUP : x < list.sink ? (x - list.pre) * GROUP : list.lo + (x - list.sink) * GROUP;
+        #pragma unroll
+        for (int h = 0; h < Sh::HALVES; ++h) {
+            load_box(dst + h * (GROUP * 128), pre ? &maps.pk : &maps.k, h * 64, j, pre ? ph : kh, pre ? 0 : kb, bar);
+            load_box(dst + Sh::TILE + h * (GROUP * 128), pre ? &maps.pv : &maps.v, h * 64, j, pre ? pvh : vh, pre ? 0 : vb, bar);
+        }
+    };
+    const int first = x0 + warp;
+    if (lane == 0 && ok) {
+        uint32_t st = stage;
+        for (int k = 0; k < STAGES && first + k * RW < x1; ++k) {
+            load(first + k * RW, st);
+            if (++st == STAGES) st = 0;
+        }
+    }
 
     // queries as the left operand's fragments: rows lane / 4 and lane / 4 + 8
     uint32_t qf[NK][4];
@@ -178,104 +227,96 @@ __global__ void __launch_bounds__(RW * 32) attention_rows_kernel(const __grid_co
             qf[kk][f] = r < rows && d < a.D
                 ? *reinterpret_cast<const uint32_t*>(static_cast<const E*>(a.q) + (int64_t)b * a.qs[0] + (int64_t)i * a.qs[1] + (int64_t)(h0 + r) * a.qs[2] + d) : 0u;
         }
-
-    auto load = [&](int64_t u, int stage) {
-        // a row of 2 NK pieces of 16 bytes, neighbouring lanes along a row: whole lines from memory
-        const uint32_t dst = ring + stage * Sh::STAGE;
-        #pragma unroll
-        for (int c = 0; c < NK; ++c) {
-            const int x = lane + 32 * c, key = x / (2 * NK), d = (x - key * (2 * NK)) * 8;
-            const int64_t y = u + key;
-            const E *kp = kb, *vp = vb;
-            const bool live = y < u1 && (uint32_t)d < a.D;
-            if (live) {
-                if (y < a.P) { kp = pk + y * a.pks[1] + d; vp = pv + y * a.pvs[1] + d; }
-                else {
-                    const int64_t z = y - a.P, j = z < ns ? z : lo + (z - ns);
-                    kp = kb + j * a.ks[2] + d; vp = vb + j * a.vs[2] + d;
-                }
-            }
-            copy16(dst + key * Sh::ROW + d * 2, kp, live);
-            copy16(dst + (GROUP + key) * Sh::ROW + d * 2, vp, live);
-        }
-    };
-
     float o[NK * 2][4];
     #pragma unroll
     for (int t = 0; t < NK * 2; ++t)
         #pragma unroll
         for (int f = 0; f < 4; ++f) o[t][f] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    const float c = a.scale_log2;
 
-    constexpr int64_t STEP = RW * GROUP;
-    const int64_t first = u0 + warp * GROUP;
-    #pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) {
-        if (first + s * STEP < u1) load(first + s * STEP, s);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    }
-    int stage = 0;
-    for (int64_t u = first; u < u1; u += STEP) {
+    for (int x = first; x < x1 && ok; x += RW) {
         {
-            const int64_t next = u + (STAGES - 1) * STEP;
-            int s = stage + STAGES - 1;
-            if (s >= STAGES) s -= STAGES;
-            if (next < u1) load(next, s);
-            asm volatile("cp.async.commit_group;" ::: "memory");
+            uint32_t it = 0;
+            while (!__all_sync(0xFFFFFFFFu, mbar_try_wait(bars + 8 * stage, phase)))
+                if (++it == POLLS) { ok = false; break; }
+            if (!ok) {
+                if (lane == 0) { *abort_flag = 1; atomicCAS(&g_tc_status, 0, 51); }
+                __syncwarp();
+                break;
+            }
         }
-        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
-        __syncwarp();
-        const uint32_t kt = ring + stage * Sh::STAGE, vt = kt + GROUP * Sh::ROW;
+        const uint32_t kt = ring + stage * Sh::STAGE, vt = kt + Sh::TILE;
+        const int run = x < list.pre ? list.P - x * GROUP : x < list.sink ? list.ns - (x - list.pre) * GROUP : list.end - list.lo - (x - list.sink) * GROUP;
+        if (run < GROUP) {                                           // values behind the run's end
+            for (int y = lane; y < (GROUP - run) * Sh::HALVES * 8; y += 32) {
+                const int key = run + y / (Sh::HALVES * 8), pc = y % (Sh::HALVES * 8);
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vt + (pc >> 3) * (GROUP * 128) + key * 128 + (pc & 7) * 16), "r"(0) : "memory");
+            }
+            __syncwarp();
+        }
         float s[2][4] = {};
         #pragma unroll
         for (int kk = 0; kk < NK; ++kk) {
             uint32_t f[4];
-            ldsm4(f, kt + ((lane & 7) + 8 * (lane >> 4)) * Sh::ROW + kk * 32 + ((lane >> 3) & 1) * 16);
+            const int row = (lane & 7) + 8 * (lane >> 4), pc = (kk & 3) * 2 + ((lane >> 3) & 1);
+            ldsm4(f, kt + (kk >> 2) * (GROUP * 128) + row * 128 + ((pc ^ (row & 7)) * 16));
             Mma<E>::run(s[0], qf[kk], f[0], f[1]);
             Mma<E>::run(s[1], qf[kk], f[2], f[3]);
         }
+        if (run < GROUP) {
+            #pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if ((e >> 2) * 8 + (lane & 3) * 2 + (e & 1) >= run) s[e >> 2][e & 3] = -INFINITY;
+        }
+        float top[2];
+        #pragma unroll
+        for (int r = 0; r < 2; ++r) top[r] = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
+        if (__any_sync(0xFFFFFFFFu, (top[0] - m[0]) * c > GROWTH || (top[1] - m[1]) * c > GROWTH)) {
+            #pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 1));
+                top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 2));
+                if (top[r] > m[r]) {
+                    const float f = exp2_fast((m[r] - top[r]) * c);
+                    m[r] = top[r];
+                    l[r] *= f;
+                    #pragma unroll
+                    for (int t = 0; t < NK * 2; ++t) { o[t][2 * r] *= f; o[t][2 * r + 1] *= f; }
+                }
+            }
+        }
         uint32_t hi[4], rest[4];
         #pragma unroll
-        for (int r = 0; r < 2; ++r) {                  // row lane / 4 + 8 r
-            float x[4], top = -INFINITY;
-            #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int64_t key = u + (e >> 1) * 8 + (lane & 3) * 2 + (e & 1);
-                x[e] = key < u1 ? s[e >> 1][2 * r + (e & 1)] * a.scale_log2 : -INFINITY;
-                top = fmaxf(top, x[e]);
-            }
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-            const float now = fmaxf(m[r], top), ref = now == -INFINITY ? 0.f : now, old = exp2_fast(m[r] - ref);
-            m[r] = now;
-            float w[4], sum = 0.f;
-            #pragma unroll
-            for (int e = 0; e < 4; ++e) { w[e] = exp2_fast(x[e] - ref); sum += w[e]; }
-            l[r] = l[r] * old + sum;
-            #pragma unroll
-            for (int t = 0; t < NK * 2; ++t) { o[t][2 * r] *= old; o[t][2 * r + 1] *= old; }
-            // the weights as two numbers of the values' type, so that their rounding does not reach the result
+        for (int r = 0; r < 2; ++r) {                                // row lane / 4 + 8 r
+            const float off = SHIFT - (m[r] == -INFINITY ? 0.f : m[r] * c);
             #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const uint32_t top2 = Mma<E>::pack(w[2 * e], w[2 * e + 1]);
-                const float2 back = Mma<E>::unpack(top2);
-                hi[2 * e + r] = top2;
-                rest[2 * e + r] = Mma<E>::pack(w[2 * e] - back.x, w[2 * e + 1] - back.y);
+                const float w0 = exp2_fast(fmaf(s[e][2 * r], c, off)), w1 = exp2_fast(fmaf(s[e][2 * r + 1], c, off));
+                l[r] += w0 + w1;
+                // the weights as two numbers of the values' type, so that their rounding does not reach the result
+                hi[2 * e + r] = Mma<E>::pack(w0, w1);
+                const float2 back = Mma<E>::unpack(hi[2 * e + r]);
+                rest[2 * e + r] = Mma<E>::pack(w0 - back.x, w1 - back.y);
             }
         }
         #pragma unroll
         for (int t = 0; t < NK; ++t) {
             uint32_t f[4];
-            ldsm4t(f, vt + ((lane & 7) + 8 * ((lane >> 3) & 1)) * Sh::ROW + t * 32 + (lane >> 4) * 16);
+            const int row = (lane & 7) + 8 * ((lane >> 3) & 1), pc = (t & 3) * 2 + (lane >> 4);
+            ldsm4t(f, vt + (t >> 2) * (GROUP * 128) + row * 128 + ((pc ^ (row & 7)) * 16));
             Mma<E>::run(o[2 * t], hi, f[0], f[1]);
             Mma<E>::run(o[2 * t], rest, f[0], f[1]);
             Mma<E>::run(o[2 * t + 1], hi, f[2], f[3]);
             Mma<E>::run(o[2 * t + 1], rest, f[2], f[3]);
         }
-        __syncwarp();                                  // the stage is refilled by the copies of the next round
-        if (++stage == STAGES) stage = 0;
+        __syncwarp();                                                // every lane has read the stage
+        if (lane == 0 && x + STAGES * RW < x1) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            load(x + STAGES * RW, stage);
+        }
+        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
     #pragma unroll
     for (int r = 0; r < 2; ++r) {
         l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 1);
@@ -292,7 +333,10 @@ __global__ void __launch_bounds__(RW * 32) attention_rows_kernel(const __grid_co
         #pragma unroll
         for (int t = 0; t < NK * 2; ++t)
             *reinterpret_cast<float2*>(js + (warp * 16 + row) * Sh::DP + t * 8 + (lane & 3) * 2) = make_float2(o[t][2 * r], o[t][2 * r + 1]);
-        if ((lane & 3) == 0) { jm[(warp * 16 + row) * 2] = m[r]; jm[(warp * 16 + row) * 2 + 1] = l[r]; }
+        if ((lane & 3) == 0) {                                       // (weights are 2^(x c - m c + SHIFT))
+            jm[(warp * 16 + row) * 2] = m[r] == -INFINITY ? m[r] : m[r] * c - SHIFT;
+            jm[(warp * 16 + row) * 2 + 1] = l[r];
+        }
     }
     __syncthreads();
     for (uint32_t x = threadIdx.x; x < rows * a.D; x += RW * 32) {
@@ -321,8 +365,16 @@ __global__ void __launch_bounds__(RW * 32) attention_rows_kernel(const __grid_co
     w0 += take;
     if (a.shared && w0 < w1) {
         if (w0 >= table[token + 1] * groups) ++token;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();                                             // the join's memory becomes the ring again
     }
+    }
+    __syncthreads();
+    if (*abort_flag) {
+        // let copies that may still be in flight land before the block's shared memory is released
+        const unsigned long long t0 = gtime_ns();
+        while (gtime_ns() - t0 < 200000ull) { }
+        __syncthreads();
     }
 }
 
@@ -392,29 +444,29 @@ __global__ void __launch_bounds__(64) attention_join_kernel(const __grid_constan
 }
 
 template <class E, int NK>
-int rows_launch(const AttnArgs& a, cudaStream_t stream)
+int rows_launch(const AttnArgs& a, const RowsMaps& maps, cudaStream_t stream)
 {
     { const int rc = ensure_dynamic_smem(attention_rows_kernel<E, NK>, RowsShape<NK>::BYTES); if (rc) return rc; }
-    HBQ_CUDA_TRY(launch_dependent(attention_rows_kernel<E, NK>, (unsigned)a.blocks, RW * 32, (size_t)RowsShape<NK>::BYTES, stream, a, (a.G + 15) / 16));
+    HBQ_CUDA_TRY(launch_dependent(attention_rows_kernel<E, NK>, (unsigned)a.blocks, RW * 32, (size_t)RowsShape<NK>::BYTES, stream, a, maps, (a.G + 15) / 16));
     HBQ_LAUNCH_CHECK("attention_rows_kernel");
     return HBQ_OK;
 }
 
 template <class E>
-int rows_type(const AttnArgs& a, cudaStream_t stream)
+int rows_type(const AttnArgs& a, const RowsMaps& maps, cudaStream_t stream)
 {
     switch ((a.D + 15) / 16) {
-        case 1: case 2: case 3: case 4: return rows_launch<E, 4>(a, stream);
-        case 5: return rows_launch<E, 5>(a, stream);
-        case 6: return rows_launch<E, 6>(a, stream);
-        case 7: return rows_launch<E, 7>(a, stream);
-        default: return rows_launch<E, 8>(a, stream);
+        case 1: case 2: case 3: case 4: return rows_launch<E, 4>(a, maps, stream);
+        case 5: return rows_launch<E, 5>(a, maps, stream);
+        case 6: return rows_launch<E, 6>(a, maps, stream);
+        case 7: return rows_launch<E, 7>(a, maps, stream);
+        default: return rows_launch<E, 8>(a, maps, stream);
     }
 }
 
 }  // namespace
 
-// Blocks of the few-row kernel; prefix: a row's list begins with it.  Shares of equal size over two blocks an SM; a block a
+// Blocks of the few-row kernel; prefix: a row's list begins with it.  Shares of equal size over the blocks that are resident at once; a block a
 // row group where there are too many tokens for the table, or where every group is a unit or two by its bounds alone.
 int attention_rows_blocks(const hbq_attention* p, bool prefix, int* shared)
 {
@@ -424,19 +476,42 @@ int attention_rows_blocks(const hbq_attention* p, bool prefix, int* shared)
     int64_t keys = p->S;
     if (p->window > 0 && p->window + p->sinks < keys) keys = p->window + p->sinks;
     if (prefix) keys += p->P;
-    const int64_t units = (keys + ROWS_UNIT - 1) / ROWS_UNIT;
-    if (tokens > RW * 64 || units <= 1) {
+    const int64_t units = (keys + RW * GROUP - 1) / (RW * GROUP) + 1;
+    if (tokens > RW * 64 || units <= 2) {
         *shared = 0;
         return groups * tokens > 0x7FFFFFFF ? -1 : (int)(groups * tokens);
     }
     *shared = 1;
     const int64_t most = units * groups * tokens;
-    return (int)(most < 2 * sms ? most : 2 * sms);
+    return (int)(most < BLOCKS_PER_SM * sms ? most : BLOCKS_PER_SM * sms);
 }
 
 int attention_rows_launch(const AttnArgs& a, int dtype, cudaStream_t stream)
 {
-    return dtype == HBQ_DTYPE_F16 ? rows_type<__half>(a, stream) : rows_type<__nv_bfloat16>(a, stream);
+    RowsMaps maps = {};
+    int rc = HBQ_OK;
+    if (a.S > 0) {
+        rc = attention_cache_map(&maps.k, a.k, dtype, a.D, GROUP, a.S, a.ks[2], a.Hkv, a.ks[1], a.B, a.ks[0]);
+        if (!rc) rc = attention_cache_map(&maps.v, a.v, dtype, a.D, GROUP, a.S, a.vs[2], a.Hkv, a.vs[1], a.B, a.vs[0]);
+    }
+    if (a.P > 0 && !rc) {
+        rc = attention_cache_map(&maps.pk, a.pk, dtype, a.D, GROUP, a.P, a.pks[1], a.Hkv, a.pks[0], 1, 0);
+        if (!rc) rc = attention_cache_map(&maps.pv, a.pv, dtype, a.D, GROUP, a.P, a.pvs[1], a.Hkv, a.pvs[0], 1, 0);
+    }
+    if (rc) return rc;
+    return dtype == HBQ_DTYPE_F16 ? rows_type<__half>(a, maps, stream) : rows_type<__nv_bfloat16>(a, maps, stream);
+}
+
+int attention_rows_status(int* host_out)
+{
+    HBQ_CUDA_TRY(cudaMemcpyFromSymbol(host_out, g_tc_status, sizeof(int)));
+    return HBQ_OK;
+}
+int attention_rows_status_reset()
+{
+    const int z = 0;
+    HBQ_CUDA_TRY(cudaMemcpyToSymbol(g_tc_status, &z, sizeof(int)));
+    return HBQ_OK;
 }
 
 int attention_join_launch(const AttnArgs& a, int dtype, cudaStream_t stream)

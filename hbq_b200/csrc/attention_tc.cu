@@ -528,23 +528,6 @@ EncodeFn encoder()
     return fn;
 }
 
-// A cache [sequences][heads][keys][D] in boxes of 128 keys by 64 values; keys beyond the last and values beyond D read as
-// zeros.  An axis whose elements are all the same ones (stride 0) is left out.
-int cache_map(CUtensorMap* map, const void* ptr, int dtype, int64_t D, int64_t keys, int64_t key_stride, int64_t heads, int64_t head_stride,
-              int64_t seqs, int64_t seq_stride)
-{
-    EncodeFn fn = encoder();
-    if (!fn) return HBQ_ERR_CUDA;
-    const auto step = [](int64_t stride, int64_t other) { return (cuuint64_t)(stride > 0 ? stride : other) * 2; };
-    const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)keys, (cuuint64_t)(head_stride > 0 ? heads : 1), (cuuint64_t)(seq_stride > 0 ? seqs : 1)};
-    const cuuint64_t strides[3] = {step(key_stride, D), step(head_stride, D), step(seq_stride, D)};
-    const cuuint32_t box[4] = {64, TILE, 1, 1}, each[4] = {1, 1, 1, 1};
-    const CUresult r = fn(map, dtype == HBQ_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr), dims,
-                          strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? HBQ_OK : HBQ_ERR_CUDA;
-}
-
 template <class E, int DP>
 int tc_launch(const CUtensorMap& mk, const CUtensorMap& mv, const AttnArgs& a, const TcTask& task, unsigned blocks, cudaStream_t stream)
 {
@@ -555,6 +538,23 @@ int tc_launch(const CUtensorMap& mk, const CUtensorMap& mv, const AttnArgs& a, c
 }
 
 }  // namespace
+
+// A cache [sequences][heads][keys][D] in boxes of `rows` keys by 64 values; keys beyond the last and values beyond D read as
+// zeros.  An axis whose elements are all the same ones (stride 0) is left out.
+int attention_cache_map(CUtensorMap* map, const void* ptr, int dtype, int64_t D, int rows, int64_t keys, int64_t key_stride, int64_t heads, int64_t head_stride,
+              int64_t seqs, int64_t seq_stride)
+{
+    EncodeFn fn = encoder();
+    if (!fn) return HBQ_ERR_CUDA;
+    const auto step = [](int64_t stride, int64_t other) { return (cuuint64_t)(stride > 0 ? stride : other) * 2; };
+    const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)keys, (cuuint64_t)(head_stride > 0 ? heads : 1), (cuuint64_t)(seq_stride > 0 ? seqs : 1)};
+    const cuuint64_t strides[3] = {step(key_stride, D), step(head_stride, D), step(seq_stride, D)};
+    const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, each[4] = {1, 1, 1, 1};
+    const CUresult r = fn(map, dtype == HBQ_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr), dims,
+                          strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? HBQ_OK : HBQ_ERR_CUDA;
+}
 
 // Into how many pieces the keys of a block's rows are cut: the count with the shortest longest SM, where a block costs its
 // key tiles and about three tiles' time to start and end, and joining pieces about four.
@@ -589,8 +589,8 @@ int attention_tc_launch(AttnArgs& a, int dtype, bool prefix, cudaStream_t stream
     task.vector_out = ((a.os[0] | a.os[1] | a.os[2]) % 8) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
     CUtensorMap mk, mv;
     const int64_t keys = prefix ? a.P : a.S;
-    { const int rc = cache_map(&mk, prefix ? a.pk : a.k, dtype, a.D, keys, ks[2], a.Hkv, ks[1], a.B, ks[0]); if (rc) return rc; }
-    { const int rc = cache_map(&mv, prefix ? a.pv : a.v, dtype, a.D, keys, vs[2], a.Hkv, vs[1], a.B, vs[0]); if (rc) return rc; }
+    { const int rc = attention_cache_map(&mk, prefix ? a.pk : a.k, dtype, a.D, TILE, keys, ks[2], a.Hkv, ks[1], a.B, ks[0]); if (rc) return rc; }
+    { const int rc = attention_cache_map(&mv, prefix ? a.pv : a.v, dtype, a.D, TILE, keys, vs[2], a.Hkv, vs[1], a.B, vs[0]); if (rc) return rc; }
     const bool wide = a.D > 64;
     if (dtype == HBQ_DTYPE_F16)
         return wide ? tc_launch<__half, 128>(mk, mv, a, task, (unsigned)blocks, stream) : tc_launch<__half, 64>(mk, mv, a, task, (unsigned)blocks, stream);
@@ -598,16 +598,19 @@ int attention_tc_launch(AttnArgs& a, int dtype, bool prefix, cudaStream_t stream
                 : tc_launch<__nv_bfloat16, 64>(mk, mv, a, task, (unsigned)blocks, stream);
 }
 
+int attention_rows_status(int* host_out);   // attention_rows.cu: that kernel's own status word
+int attention_rows_status_reset();
+
 int attention_tc_status(int* host_out)
 {
     HBQ_CUDA_TRY(cudaMemcpyFromSymbol(host_out, g_tc_status, sizeof(int)));
-    return HBQ_OK;
+    return *host_out ? HBQ_OK : attention_rows_status(host_out);
 }
 int attention_tc_status_reset()
 {
     const int z = 0;
     HBQ_CUDA_TRY(cudaMemcpyToSymbol(g_tc_status, &z, sizeof(int)));
-    return HBQ_OK;
+    return attention_rows_status_reset();
 }
 
 }  // namespace hbq
