@@ -50,10 +50,10 @@ Plan plan_of(const hbq_attention* p)
     else if (!c.prefix_tc || p->S > 0) c.blocks = attention_rows_blocks(p, !alone, &c.shared);
     c.parts = c.prefix + c.own + (c.prefix_tc && c.blocks ? 1 : 0);
     if (c.parts == 1) c.parts = 0;
-    const auto up = [](int64_t n) { return (n + 15) / 16 * 16; };
+    const auto up = [](int64_t n) { return (n + 31) / 32 * 32; };
     c.part_bytes = up(p->B * p->L * p->H * c.parts * (p->D + 2) * 4);
     if (c.shared) {
-        c.table_bytes = up((p->B * p->L + 1) * 8);
+        c.table_bytes = up(p->B * p->L * p->Hkv * ((p->H / p->Hkv + 15) / 16) * 8);
         c.slot_bytes = up((int64_t)c.blocks * 2 * 16 * (p->D + 2) * 4);
     }
     return c;
@@ -80,11 +80,11 @@ int attention_run(const hbq_attention* p, void* workspace, int64_t workspace_byt
     const Plan c = plan_of(p);
     if (c.blocks < 0) return HBQ_ERR_UNSUPPORTED;
     const int64_t need = c.bytes();
-    if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))) return HBQ_ERR_WORKSPACE;
+    if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 31))) return HBQ_ERR_WORKSPACE;
     a.parts = c.parts; a.blocks = c.blocks; a.shared = c.shared;
     char* ws = static_cast<char*>(workspace);
     a.part = reinterpret_cast<float*>(ws);
-    a.table = reinterpret_cast<int64_t*>(ws + c.part_bytes);
+    a.table = reinterpret_cast<int2*>(ws + c.part_bytes);
     a.slots = reinterpret_cast<float*>(ws + c.part_bytes + c.table_bytes);
     if (c.prefix_tc) {
         a.nsplit = c.prefix;

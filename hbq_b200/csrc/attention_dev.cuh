@@ -18,7 +18,7 @@ struct AttnArgs {
     int parts, part0;
     // The few-row kernel's division of work: `blocks` blocks of equal shares; its table and slots in the workspace.
     int blocks, shared;                                      // shared: shares may begin and end inside a row group
-    int64_t* table;                                          // [B * L + 1] units before each token
+    int2* table;                                             // of each row group: its first block and how many; 0: undivided
     float* slots;                                            // [blocks][2][16][D] sums, then [blocks][2][16] (maximum, weight)
 };
 

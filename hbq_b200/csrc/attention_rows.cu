@@ -153,14 +153,12 @@ __global__ void __launch_bounds__(RW * 32, BLOCKS_PER_SM) attention_rows_kernel(
     grid_dependency_wait();
     dependents_may_start();
     const uint32_t groups = a.Hkv * tiles, tokens = a.B * a.L;       // row groups of a token
-    int64_t w0, w1;                                                  // this block's share of the units
+    int64_t w0, w1, total = 1, takers = 1;                           // this block's share of the units
     uint32_t token;
     if (a.shared) {
         count_units(a, table);
-        if (blockIdx.x == 0)
-            for (uint32_t r = threadIdx.x; r <= tokens; r += RW * 32) a.table[r] = table[r];
-        const int64_t total = table[tokens] * groups;
-        const int64_t takers = rows_takers(a, total);
+        total = table[tokens] * groups;
+        takers = rows_takers(a, total);
         if (blockIdx.x >= takers) return;
         w0 = total * blockIdx.x / takers; w1 = total * (blockIdx.x + 1) / takers;
         uint32_t low = 0, high = tokens;                             // the last token that begins at or before w0
@@ -191,6 +189,8 @@ __global__ void __launch_bounds__(RW * 32, BLOCKS_PER_SM) attention_rows_kernel(
         x0 = (int)off * RW;
         x1 = (int)min((int64_t)list.steps, (off + take) * RW);
         slot = take == units ? -1 : off > 0 ? 0 : 1;
+        if (off == 0 && threadIdx.x == 0)
+            a.table[(int64_t)token * groups + g] = make_int2(blockIdx.x, slot < 0 ? 0 : rows_owner(w0 + units - 1, total, takers) - (int)blockIdx.x + 1);
     } else g = blockIdx.x - token * groups;
     const uint32_t hk = g / tiles, g0 = (g - hk * tiles) * 16, rows = min(16u, a.G - g0), h0 = hk * a.G + g0;
     const int kh = a.ks[1] > 0 ? (int)hk : 0, kb = a.ks[0] > 0 ? (int)b : 0, vh = a.vs[1] > 0 ? (int)hk : 0, vb = a.vs[0] > 0 ? (int)b : 0;
@@ -378,31 +378,28 @@ __global__ void __launch_bounds__(RW * 32, BLOCKS_PER_SM) attention_rows_kernel(
     }
 }
 
-// One warp joins a row's parts: the tensor-core kernel's, and the few-row kernel's part or slots.  Maxima, then weights and
-// sums relative to the largest.
-template <class E>
-__global__ void __launch_bounds__(64) attention_join_kernel(const __grid_constant__ AttnArgs a, uint32_t tiles)
+// W warps join a row's parts: the tensor-core kernel's, and the few-row kernel's part or slots.  Maxima, then weights and
+// sums relative to the largest.  A chain of dependent loads, bound by their latency: the blocks of a group come from its
+// table entry, and with few rows four warps share a row's parts (8 rows of 37 parts: 8.4 -> 5 us).
+template <class E, int W>
+__global__ void __launch_bounds__(128) attention_join_kernel(const __grid_constant__ AttnArgs a, uint32_t tiles)
 {
+    __shared__ float sums[W > 1 ? W : 1][128], weights[W > 1 ? W : 1];
     grid_dependency_wait();
     dependents_may_start();
-    const int lane = threadIdx.x & 31;
-    const int64_t row = (int64_t)blockIdx.x * 2 + (threadIdx.x >> 5);
-    if (row >= (int64_t)a.B * a.L * a.H) return;
-    const int64_t token = row / a.H;
-    const uint32_t h = (uint32_t)(row - token * a.H);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = W > 1 ? warp : 0;
+    const uint32_t row = W > 1 ? blockIdx.x : blockIdx.x * 4 + warp;
+    if (row >= a.B * a.L * a.H) return;
+    const uint32_t token = row / a.H, h = row - token * a.H;
     int first = 0, count = a.parts, listed = a.parts, gr = 0;       // parts 0 .. listed - 1 lie in the row's list, the rest in slots
     if (a.shared) {
-        const uint32_t hk = h / a.G, gg = h - hk * a.G, groups = a.Hkv * tiles;
+        const uint32_t hk = h / a.G, gg = h - hk * a.G;
         gr = (int)(gg & 15);
-        const int64_t* table = behind_wait(a.table);
-        const int64_t begin = table[token], units = table[token + 1] - begin, total = table[(int64_t)a.B * a.L] * groups;
-        const int64_t s0 = begin * groups + (int64_t)(hk * tiles + gg / 16) * units;
-        const int64_t takers = rows_takers(a, total);
-        first = rows_owner(s0, total, takers);
-        const int last = rows_owner(s0 + units - 1, total, takers);
-        if (first < last) {
+        const int2 blocks = behind_wait(a.table)[(int64_t)token * (a.Hkv * tiles) + hk * tiles + gg / 16];
+        first = blocks.x;
+        if (blocks.y > 0) {
             if (listed > 0) --listed;                                // (the entry for an undivided group is not in use)
-            count = listed + last - first + 1;
+            count = listed + blocks.y;
         } else if (a.parts == 0) return;                             // undivided: written already
     }
     const auto weight_of = [&](int s) { return s < listed ? *part_weight(a, row, s) : *slot_weight(a, first + s - listed, s == listed, gr); };
@@ -417,30 +414,56 @@ __global__ void __launch_bounds__(64) attention_join_kernel(const __grid_constan
     const float ref = top == -INFINITY ? 0.f : top;
     float weight = 0.f, sum[4] = {};
     const bool in = lane * 4 < (int)a.D;
-    for (int s0 = 0; s0 < count; s0 += 32) {
+    for (int s0 = sub; s0 < count; s0 += 32 * W) {                   // this warp's parts: s0, s0 + W, ...
         float f = 0.f;
-        if (s0 + lane < count) {
-            const float2 ml = weight_of(s0 + lane);
+        if (s0 + lane * W < count) {
+            const float2 ml = weight_of(s0 + lane * W);
             if (ml.y != 0.f) { f = exp2_fast(ml.x - ref); weight = fmaf(ml.y, f, weight); }
         }
-        const int end = min(32, count - s0);
-        #pragma unroll 4
+        const int end = min(32, (count - s0 + W - 1) / W);
+        #pragma unroll 8
         for (int s = 0; s < end; ++s) {
             const float g = __shfl_sync(0xFFFFFFFFu, f, s);
             if (g != 0.f && in) {                                    // an empty part's sums are not looked at (a NaN is no zero)
-                const float4 x = *reinterpret_cast<const float4*>(sum_of(s0 + s) + lane * 4);
+                const float4 x = *reinterpret_cast<const float4*>(sum_of(s0 + s * W) + lane * 4);
                 sum[0] = fmaf(x.x, g, sum[0]); sum[1] = fmaf(x.y, g, sum[1]); sum[2] = fmaf(x.z, g, sum[2]); sum[3] = fmaf(x.w, g, sum[3]);
             }
         }
     }
     #pragma unroll
     for (int k = 16; k; k >>= 1) weight += __shfl_xor_sync(0xFFFFFFFFu, weight, k);
-    const int64_t b = token / a.L, i = token - b * a.L;
+    if (W > 1) {
+        #pragma unroll
+        for (int e = 0; e < 4; ++e) sums[sub][lane * 4 + e] = sum[e];
+        if (lane == 0) weights[sub] = weight;
+        __syncthreads();
+        if (warp > 0) return;
+        #pragma unroll
+        for (int w = 1; w < W; ++w) {
+            weight += weights[w];
+            #pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] += sums[w][lane * 4 + e];
+        }
+    }
+    const uint32_t b = token / a.L, i = token - b * a.L;
     if (in) {
         #pragma unroll
         for (int e = 0; e < 4; ++e)
-            Mma<E>::store(a.out, b * a.os[0] + i * a.os[1] + h * a.os[2] + lane * 4 + e, weight == 0.f ? 0.f : sum[e] / weight);
+            Mma<E>::store(a.out, (int64_t)b * a.os[0] + (int64_t)i * a.os[1] + (int64_t)h * a.os[2] + lane * 4 + e, weight == 0.f ? 0.f : sum[e] / weight);
     }
+}
+
+template <class E>
+int join_launch(const AttnArgs& a, cudaStream_t stream)
+{
+    const int64_t rows = (int64_t)a.B * a.L * a.H;
+    if (rows > 0x7FFFFFFFll) return HBQ_ERR_UNSUPPORTED;
+    const uint32_t tiles = (a.G + 15) / 16;
+    // (64 x 32 rows of a few parts each, and fewer, are less than the SMs hold at once)
+    if (rows <= 4096) HBQ_CUDA_TRY(launch_dependent(attention_join_kernel<E, 4>, (unsigned)rows, 128, 0, stream, a, tiles));
+    else HBQ_CUDA_TRY(launch_dependent(attention_join_kernel<E, 1>, (unsigned)((rows + 3) / 4), 128, 0, stream, a, tiles));
+    HBQ_LAUNCH_CHECK("attention_join_kernel");
+    return HBQ_OK;
 }
 
 template <class E, int NK>
@@ -516,13 +539,7 @@ int attention_rows_status_reset()
 
 int attention_join_launch(const AttnArgs& a, int dtype, cudaStream_t stream)
 {
-    const int64_t blocks = ((int64_t)a.B * a.L * a.H + 1) / 2;
-    if (blocks > 0x7FFFFFFFll) return HBQ_ERR_UNSUPPORTED;
-    const uint32_t tiles = (a.G + 15) / 16;
-    if (dtype == HBQ_DTYPE_F16) HBQ_CUDA_TRY(launch_dependent(attention_join_kernel<__half>, (unsigned)blocks, 64, 0, stream, a, tiles));
-    else HBQ_CUDA_TRY(launch_dependent(attention_join_kernel<__nv_bfloat16>, (unsigned)blocks, 64, 0, stream, a, tiles));
-    HBQ_LAUNCH_CHECK("attention_join_kernel");
-    return HBQ_OK;
+    return dtype == HBQ_DTYPE_F16 ? join_launch<__half>(a, stream) : join_launch<__nv_bfloat16>(a, stream);
 }
 
 }  // namespace hbq

@@ -490,8 +490,10 @@ __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_const
                         }
                     } else {
                         #pragma unroll
-                        for (int e = 0; e < 32; e += 4)
-                            if (32 * k + e < (int)a.D) *reinterpret_cast<float4*>(part + 32 * k + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                        for (int e = 0; e < 32; e += 8)          // whole sectors
+                            if (32 * k + e < (int)a.D)
+                                asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(part + 32 * k + e), "f"(o[e]), "f"(o[e + 1]),
+                                             "f"(o[e + 2]), "f"(o[e + 3]), "f"(o[e + 4]), "f"(o[e + 5]), "f"(o[e + 6]), "f"(o[e + 7]) : "memory");
                     }
                 }
                 if (!direct && r < rend)
