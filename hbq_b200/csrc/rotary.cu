@@ -4,7 +4,7 @@
 //   (u, v) -> factor * (u cos a - v sin a, v cos a + u sin a),   a = position * inv_freq[i], for each pair i
 //
 // Bound by memory: each value is read once and written once.  A position's angles are the same for all of its heads, so a
-// block computes them once into shared memory: the product and its reduction to a part of a turn in 64 bits (at position
+// warp computes them once for many: the product and its reduction to a part of a turn in 64 bits (at position
 // 10^6 an angle in 32 bits is off by 0.06), cosine and sine of that part in 32 bits.  A table of them would be read
 // from memory in their place and has to be kept for every position.
 #include "common.cuh"
@@ -24,13 +24,13 @@ struct RotaryArgs {
     const double* inv_freq;
     const void* positions;
     int64_t pb, pt, tokens;        // tokens = B * T
-    uint32_t T, heads0, heads, D, rot, groups;
+    uint32_t T, heads0, heads, D, rot;
     int interleaved, positions_64;
-    float factor, eps;
-    int tokens_per_block;
+    float factor, eps, inv_D;
+    int many;                      // a warp per token
 };
 
-constexpr int WARPS = 8;
+constexpr int WARPS = 4;
 
 template <class E> struct Pair;
 template <> struct Pair<__half> {
@@ -64,115 +64,159 @@ __device__ __forceinline__ void rotate(float& u, float& v, float2 cs)
     v = fmaf(v, cs.x, u * cs.y);
     u = r;
 }
-__device__ __forceinline__ int64_t position_of(const RotaryArgs& a, int64_t token)
+__device__ __forceinline__ int64_t position_of(const RotaryArgs& a, int64_t b, int64_t t)
 {
-    const int64_t b = token / a.T, t = token - b * a.T, i = b * a.pb + t * a.pt;
+    const int64_t i = b * a.pb + t * a.pt;
     return a.positions_64 ? static_cast<const int64_t*>(a.positions)[i] : static_cast<const int32_t*>(a.positions)[i];
+}
+
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+    float2 d;
+    asm("{ .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n fma.rn.f32x2 z, x, y, z;\n mov.b64 {%0, %1}, z; }"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+    float2 d;
+    asm("{ .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x; }"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+// A lane's two runs as first and second values of its eight pairs, two pairs to a register pair (the packed 32-bit operations
+// halve the instructions, which bound the norm: 302 a group of heads before)
+template <class E>
+__device__ __forceinline__ void unpack(uint4 r0, uint4 r1, bool apart, float2 (&u)[4], float2 (&v)[4])
+{
+    const uint32_t x[4] = {r0.x, r0.y, r0.z, r0.w}, y[4] = {r1.x, r1.y, r1.z, r1.w};
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (apart) { u[i] = Pair<E>::up(x[i]); v[i] = Pair<E>::up(y[i]); }
+        else {
+            const float2 p = Pair<E>::up(i < 2 ? x[2 * i] : y[2 * i - 4]), q = Pair<E>::up(i < 2 ? x[2 * i + 1] : y[2 * i - 3]);
+            u[i] = make_float2(p.x, q.x);
+            v[i] = make_float2(p.y, q.y);
+        }
+    }
 }
 
 // Heads whose length and turning part are multiples of 16: a lane holds two runs of 8 values, which the rotation pairs
 // with one another (runs c and c + rot / 16 of the half layout, neighbours of the interleaved one), so that a pair never
 // leaves its lane; LANES lanes share a head and 32 / LANES heads a warp.  Each lane needs the 8 angles from 8 c on.
-// A block takes `tokens_per_block` tokens: eight where there are many, so that a warp keeps one token's angles in
-// registers over all its heads; one where there are few, its heads spread over the warps and over blockIdx.y.
+// A warp has one token, whose angles it computes for itself; with many tokens it walks over all of the token's heads, with
+// few a token's heads are spread over the warps of its blocks (blockIdx.y).
+//
+// Bytes in flight are what it needs: a warp's next heads are loaded before it works on the present ones, and its first ones
+// before the block's angles are known (16384 tokens of 32 heads of 128: 47 us, 5.7 TB/s; 32 + 8 heads with
+// the norm: 67 us, 5.0 TB/s).
 template <class E, int LANES, bool NORM>
-__global__ void __launch_bounds__(WARPS * 32) rotary_kernel(const __grid_constant__ RotaryArgs a)
+__global__ void __launch_bounds__(WARPS * 32, 6) rotary_kernel(const __grid_constant__ RotaryArgs a)
 {
-    extern __shared__ float2 angles[];             // [tokens_per_block][rot / 2]
+    __shared__ float2 block_angles[WARPS][128];    // [warp][rot / 2]
     grid_dependency_wait();
     dependents_may_start();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane & (LANES - 1), sub = lane / LANES;
-    const uint32_t half = a.rot / 2, tpb = (uint32_t)a.tokens_per_block;
-    const int64_t token0 = (int64_t)blockIdx.x * tpb;
-    const uint32_t here = (uint32_t)min((int64_t)tpb, a.tokens - token0);
-    const double* freq = behind_wait(a.inv_freq);
-    for (uint32_t i = threadIdx.x; i < here * half; i += WARPS * 32) {
-        const uint32_t t = i / half;
-        angles[i] = turn(position_of(a, token0 + t), freq[i - t * half], a.factor);
-    }
-    __syncthreads();
-
+    const uint32_t half = a.rot / 2;
     const bool in_head = (uint32_t)c * 16 < a.D, turns = (uint32_t)c * 16 < a.rot;
+    // `apart`: pair i of the lane is (first run's i, second run's i); else its values are neighbours
+    const bool apart = !a.interleaved;
     uint32_t d0, d1;                               // where the lane's two runs begin
     if (a.interleaved || !turns) { d0 = 16 * c; d1 = d0 + 8; }
     else { d0 = 8 * c; d1 = d0 + half; }
-    float w[2][16];
-    if (NORM) {
-        #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const void* wp = a.x[j].weight;
-            #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                uint4 u = make_uint4(0, 0, 0, 0);
-                if (in_head && wp) u = *reinterpret_cast<const uint4*>(static_cast<const E*>(wp) + (r ? d1 : d0));
-                const uint32_t ww[4] = {u.x, u.y, u.z, u.w};
+
+    // this warp's token, and its groups of heads: first the queries', then the keys'
+    constexpr uint32_t PER = 32 / LANES;
+    const uint32_t token = a.many ? blockIdx.x * WARPS + warp : blockIdx.x, step = a.many ? 1 : WARPS * gridDim.y;
+    const bool any = token < (uint32_t)a.tokens;
+    const uint32_t b = token / a.T, t = token - b * a.T;
+    uint32_t g = a.many ? 0 : blockIdx.y * WARPS + warp;
+
+    struct Item { uint4 u0, u1; E* out; };         // out: null for lanes without a head
+    const auto load = [&](const HeadsArg& x, const E* from, E* to, uint32_t heads, uint32_t group) {
+        Item v = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0), nullptr};
+        const uint32_t h = group * PER + sub;
+        if (h < heads && in_head) {
+            const E* p = from + (int64_t)(int)h * (int)x.sh;
+            v.u0 = *reinterpret_cast<const uint4*>(p + d0);
+            v.u1 = *reinterpret_cast<const uint4*>(p + d1);
+            v.out = to + (int64_t)(int)h * (int)x.oh;
+        }
+        return v;
+    };
+    const double* freq = behind_wait(a.inv_freq);
+    float2 cs[4], neg[4];                          // cosines and negated sines of the lane's pairs, two and two
+    bool ready = false;
+    #pragma unroll 1
+    for (int j = 0; j < 2; ++j) {
+        const HeadsArg& x = a.x[j];
+        const uint32_t heads = j ? a.heads - a.heads0 : a.heads0, groups = (heads + PER - 1) / PER;
+        const E* from = static_cast<const E*>(x.data) + (int64_t)b * x.sb + (int64_t)t * x.st;
+        E* to = static_cast<E*>(x.out) + (int64_t)b * x.ob + (int64_t)t * x.ot;
+        Item next = load(x, from, to, any ? heads : 0, g);
+        float2 wu[4], ww[4];                       // the weights, as the values below
+        if (NORM) {
+            uint4 u0 = make_uint4(0, 0, 0, 0), u1 = u0;
+            if (in_head && g < groups) {
+                u0 = *reinterpret_cast<const uint4*>(static_cast<const E*>(x.weight) + d0);
+                u1 = *reinterpret_cast<const uint4*>(static_cast<const E*>(x.weight) + d1);
+            }
+            unpack<E>(u0, u1, apart, wu, ww);
+        }
+        if (!ready) {                              // (the first loads are on their way)
+            ready = true;
+            float2* angles = block_angles[warp];
+            if (any) {
+                const int64_t position = position_of(a, b, t);
+                for (uint32_t i = lane; i < half; i += 32) angles[i] = turn(position, freq[i], a.factor);
+            }
+            __syncwarp();
+            if (turns && any) {
                 #pragma unroll
-                for (int p = 0; p < 4; ++p) {
-                    const float2 f = Pair<E>::up(ww[p]);
-                    w[j][8 * r + 2 * p] = f.x; w[j][8 * r + 2 * p + 1] = f.y;
+                for (int i = 0; i < 4; ++i) {
+                    const float2 p = angles[8 * c + 2 * i], q = angles[8 * c + 2 * i + 1];
+                    cs[i] = make_float2(p.x, q.x);
+                    neg[i] = make_float2(-p.y, -q.y);
                 }
             }
         }
-    }
-    float2 cs[8];
-    uint32_t cur = 0xFFFFFFFFu;
-    int64_t b = 0, t = 0;
-    constexpr uint32_t PER = 32 / LANES;
-    const uint32_t items = here * a.groups, stride = WARPS * gridDim.y;
-    for (uint32_t it = blockIdx.y * WARPS + warp; it < items; it += stride) {
-        // (tokens of a block innermost: with eight of them a warp keeps its own)
-        const uint32_t g = it / here, tk = it - g * here;
-        if (tk != cur) {
-            cur = tk;
-            b = (token0 + tk) / a.T; t = token0 + tk - b * a.T;
+        for (; g < groups && any; g += step) {
+            const Item cur = next;
+            next = load(x, from, to, heads, g + step);
+            float2 u[4], v[4];
+            unpack<E>(cur.u0, cur.u1, apart, u, v);
+            if (NORM) {
+                float2 q = make_float2(0.f, 0.f);
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) { q = fma2(u[i], u[i], q); q = fma2(v[i], v[i], q); }
+                float s = q.x + q.y;
+                #pragma unroll
+                for (int m = LANES / 2; m; m >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, m);
+                s = rsqrtf(fmaf(s, a.inv_D, a.eps));
+                const float2 ss = make_float2(s, s);
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) { u[i] = mul2(u[i], mul2(ss, wu[i])); v[i] = mul2(v[i], mul2(ss, ww[i])); }
+            }
             if (turns) {
                 #pragma unroll
-                for (int i = 0; i < 8; ++i) cs[i] = angles[tk * half + 8 * c + i];
+                for (int i = 0; i < 4; ++i) {
+                    const float2 r = fma2(u[i], cs[i], mul2(v[i], neg[i]));
+                    v[i] = fma2(v[i], cs[i], mul2(u[i], make_float2(-neg[i].x, -neg[i].y)));
+                    u[i] = r;
+                }
+            }
+            if (cur.out) {
+                if (apart) {
+                    *reinterpret_cast<uint4*>(cur.out + d0) = make_uint4(Pair<E>::down(u[0].x, u[0].y), Pair<E>::down(u[1].x, u[1].y), Pair<E>::down(u[2].x, u[2].y), Pair<E>::down(u[3].x, u[3].y));
+                    *reinterpret_cast<uint4*>(cur.out + d1) = make_uint4(Pair<E>::down(v[0].x, v[0].y), Pair<E>::down(v[1].x, v[1].y), Pair<E>::down(v[2].x, v[2].y), Pair<E>::down(v[3].x, v[3].y));
+                } else {
+                    *reinterpret_cast<uint4*>(cur.out + d0) = make_uint4(Pair<E>::down(u[0].x, v[0].x), Pair<E>::down(u[0].y, v[0].y), Pair<E>::down(u[1].x, v[1].x), Pair<E>::down(u[1].y, v[1].y));
+                    *reinterpret_cast<uint4*>(cur.out + d1) = make_uint4(Pair<E>::down(u[2].x, v[2].x), Pair<E>::down(u[2].y, v[2].y), Pair<E>::down(u[3].x, v[3].x), Pair<E>::down(u[3].y, v[3].y));
+                }
             }
         }
-        const uint32_t h = g * PER + sub;
-        const bool second = h >= a.heads0, live = h < a.heads && in_head;
-        const HeadsArg& x = a.x[second ? 1 : 0];
-        const int64_t hh = second ? h - a.heads0 : h;
-        uint4 u0 = make_uint4(0, 0, 0, 0), u1 = u0;
-        if (live) {
-            const E* p = static_cast<const E*>(x.data) + b * x.sb + t * x.st + hh * x.sh;
-            u0 = *reinterpret_cast<const uint4*>(p + d0);
-            u1 = *reinterpret_cast<const uint4*>(p + d1);
-        }
-        float v[16];
-        {
-            const uint32_t uu[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
-            #pragma unroll
-            for (int p = 0; p < 8; ++p) {
-                const float2 f = Pair<E>::up(uu[p]);
-                v[2 * p] = f.x; v[2 * p + 1] = f.y;
-            }
-        }
-        if (NORM) {
-            float s = 0.f;
-            #pragma unroll
-            for (int i = 0; i < 16; ++i) s = fmaf(v[i], v[i], s);
-            #pragma unroll
-            for (int m = LANES / 2; m; m >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, m);
-            s = rsqrtf(s / (float)a.D + a.eps);
-            #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] *= s * (second ? w[1][i] : w[0][i]);
-        }
-        if (turns) {
-            if (a.interleaved) {
-                #pragma unroll
-                for (int i = 0; i < 8; ++i) rotate(v[2 * i], v[2 * i + 1], cs[i]);
-            } else {
-                #pragma unroll
-                for (int i = 0; i < 8; ++i) rotate(v[i], v[8 + i], cs[i]);
-            }
-        }
-        if (live) {
-            E* o = static_cast<E*>(x.out) + b * x.ob + t * x.ot + hh * x.oh;
-            *reinterpret_cast<uint4*>(o + d0) = make_uint4(Pair<E>::down(v[0], v[1]), Pair<E>::down(v[2], v[3]), Pair<E>::down(v[4], v[5]), Pair<E>::down(v[6], v[7]));
-            *reinterpret_cast<uint4*>(o + d1) = make_uint4(Pair<E>::down(v[8], v[9]), Pair<E>::down(v[10], v[11]), Pair<E>::down(v[12], v[13]), Pair<E>::down(v[14], v[15]));
-        }
+        g = g > groups ? g - groups : 0;           // among the keys' groups
+        if (a.many) g = 0;
     }
 }
 
@@ -201,7 +245,7 @@ __global__ void __launch_bounds__(WARPS * 32) rotary_any_kernel(const __grid_con
             for (int m = 16; m; m >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, m);
             s = rsqrtf(s / (float)a.D + a.eps);
         }
-        const int64_t position = position_of(a, token);
+        const int64_t position = position_of(a, b, t);
         for (uint32_t p = lane; p < half; p += 32) {
             const uint32_t d0 = a.interleaved ? 2 * p : p, d1 = a.interleaved ? d0 + 1 : p + half;
             float u = Pair<E>::up1(x.data, in + d0), v = Pair<E>::up1(x.data, in + d1);
@@ -223,13 +267,11 @@ template <class E, int LANES, bool NORM>
 int launch_lanes(RotaryArgs& a, int sms, cudaStream_t stream)
 {
     constexpr int PER = 32 / LANES;
-    a.groups = (a.heads + PER - 1) / PER;
-    a.tokens_per_block = a.tokens >= (int64_t)sms * 16 ? 8 : 1;
-    const int64_t blocks = (a.tokens + a.tokens_per_block - 1) / a.tokens_per_block;
-    if (blocks > 0x7FFFFFFFll) return HBQ_ERR_UNSUPPORTED;
-    const unsigned split = a.tokens_per_block > 1 ? 1u : (a.groups + WARPS - 1) / WARPS;
-    HBQ_CUDA_TRY(launch_dependent(rotary_kernel<E, LANES, NORM>, dim3((unsigned)blocks, split), WARPS * 32,
-                                  (size_t)a.tokens_per_block * (a.rot / 2) * sizeof(float2), stream, a));
+    const uint32_t groups = (a.heads0 + PER - 1) / PER + (a.heads - a.heads0 + PER - 1) / PER;
+    a.many = a.tokens >= (int64_t)sms * 16;
+    const int64_t blocks = a.many ? (a.tokens + WARPS - 1) / WARPS : a.tokens;
+    const unsigned split = a.many ? 1u : (groups + WARPS - 1) / WARPS;
+    HBQ_CUDA_TRY(launch_dependent(rotary_kernel<E, LANES, NORM>, dim3((unsigned)blocks, split), WARPS * 32, 0, stream, a));
     HBQ_LAUNCH_CHECK("rotary_kernel");
     return HBQ_OK;
 }
@@ -251,10 +293,11 @@ int launch_type(RotaryArgs& a, bool runs, cudaStream_t stream)
     return HBQ_OK;
 }
 
-// The vector kernel's terms for one tensor: 16-byte runs everywhere.
+// The vector kernel's terms for one tensor: 16-byte runs everywhere, neighbouring heads less than 2^31 values apart.
 bool in_runs(const hbq_heads* x)
 {
     int64_t s = 0;
+    if (x->stride[2] > 0x7FFFFFFF || x->out_stride[2] > 0x7FFFFFFF || x->stride[2] < 0 || x->out_stride[2] < 0) return false;
     for (int i = 0; i < 3; ++i) s |= x->stride[i] | x->out_stride[i];
     return (s % 8) == 0 && ((reinterpret_cast<uintptr_t>(x->data) | reinterpret_cast<uintptr_t>(x->out) | reinterpret_cast<uintptr_t>(x->weight)) & 15) == 0;
 }
@@ -273,7 +316,7 @@ int rotary_launch(const hbq_heads* q, const hbq_heads* k, const hbq_rotary* r, i
     if (D > (1 << 20) || heads > (1 << 20) || T > 0x7FFFFFFFll || B > 0x7FFFFFFFll) return HBQ_ERR_UNSUPPORTED;
     RotaryArgs a = {};
     const hbq_heads* x[2] = {q, k};
-    bool runs = (D % 16) == 0 && D <= 256 && (r->rot % 16) == 0;
+    bool runs = (D % 16) == 0 && D <= 256 && (r->rot % 16) == 0 && B * T <= 0x7FFFFFFFll;
     for (int i = 0; i < 2; ++i) {
         if (!x[i] || x[i]->heads == 0) continue;
         if (!x[i]->data || !x[i]->out || (norm && !x[i]->weight)) return HBQ_ERR_ARG;
@@ -284,7 +327,7 @@ int rotary_launch(const hbq_heads* q, const hbq_heads* k, const hbq_rotary* r, i
     a.inv_freq = r->inv_freq; a.positions = r->positions; a.pb = r->pos_stride[0]; a.pt = r->pos_stride[1];
     a.tokens = B * T; a.T = (uint32_t)T; a.heads0 = (uint32_t)q->heads; a.heads = (uint32_t)heads;
     a.D = (uint32_t)D; a.rot = (uint32_t)r->rot; a.interleaved = r->interleaved != 0; a.positions_64 = r->positions_64 != 0;
-    a.factor = r->factor; a.eps = eps;
+    a.factor = r->factor; a.eps = eps; a.inv_D = 1.f / (float)D;
     if (dtype == HBQ_DTYPE_F16) return norm ? launch_type<__half, true>(a, runs, stream) : launch_type<__half, false>(a, runs, stream);
     return norm ? launch_type<__nv_bfloat16, true>(a, runs, stream) : launch_type<__nv_bfloat16, false>(a, runs, stream);
 }
