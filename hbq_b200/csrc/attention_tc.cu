@@ -315,21 +315,23 @@ __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_const
         float m = -INFINITY, l = 0.f;
         const float c = a.scale_log2;
         if (nt > 0) {
-            // queries of this warp's 32 rows: 16-byte pieces, neighbouring lanes along a row
+            // queries of this warp's 32 rows: 16-byte pieces, neighbouring lanes along a row, all loads at once (four at a time
+            // cost a block of few keys 2 us); a row's address comes from the lane that owns the row
             constexpr int PIECES = DP / 8;
-            #pragma unroll 4
-            for (int x = lane; x < 32 * PIECES; x += 32) {
-                const int row = x / PIECES, pc = x - row * PIECES;
-                const uint32_t q = warp * 32 + row, at = r0 + q;
-                uint4 u = make_uint4(0, 0, 0, 0);
-                if (at < rend && pc * 8 < (int)a.D) {
-                    uint32_t rr = at, bb = group;
-                    if (task.prefix) { bb = rr / (a.L * a.G); rr -= bb * (a.L * a.G); }
-                    const uint32_t ii = rr / a.G, hh = hk * a.G + (rr - ii * a.G);
-                    u = *reinterpret_cast<const uint4*>(static_cast<const E*>(a.q) + (int64_t)bb * a.qs[0] + (int64_t)ii * a.qs[1] + (int64_t)hh * a.qs[2] + pc * 8);
-                }
+            const int64_t at = r < rend ? (int64_t)b * a.qs[0] + (int64_t)i * a.qs[1] + (int64_t)h * a.qs[2] : -1;
+            uint4 x[PIECES];
+            #pragma unroll
+            for (int k = 0; k < PIECES; ++k) {
+                const int row = k * (32 / PIECES) + lane / PIECES, pc = lane % PIECES;
+                const int64_t from = __shfl_sync(0xFFFFFFFFu, at, row);
+                x[k] = make_uint4(0, 0, 0, 0);
+                if (from >= 0 && pc * 8 < (int)a.D) x[k] = *reinterpret_cast<const uint4*>(static_cast<const E*>(a.q) + from + pc * 8);
+            }
+            #pragma unroll
+            for (int k = 0; k < PIECES; ++k) {
+                const uint32_t q = warp * 32 + k * (32 / PIECES) + lane / PIECES, pc = lane % PIECES;
                 const uint32_t dst = qs + (pc >> 3) * (2 * TILE * 128) + q * 128 + (((pc & 7) ^ (q & 7)) * 16);
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(x[k].x), "r"(x[k].y), "r"(x[k].z), "r"(x[k].w) : "memory");
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -475,17 +477,24 @@ __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_const
                     }
                     if (r >= rend) {
                     } else if (direct) {
+                        uint32_t w[16];
                         #pragma unroll
-                        for (int e = 0; e < 32; e += 8) {
-                            if (32 * k + e < (int)a.D) {
-                                uint32_t w[4];
+                        for (int z = 0; z < 16; ++z) w[z] = Word<E>::pack(o[2 * z] * f, o[2 * z + 1] * f);
+                        #pragma unroll
+                        for (int e = 0; e < 32; e += 16) {
+                            E* to = out + 32 * k + e;
+                            const uint32_t* v = w + e / 2;
+                            const int left = (int)a.D - 32 * k - e;
+                            if (task.vector_out == 2 && left >= 16)  // whole sectors
+                                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                                             "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+                            else if (task.vector_out) {
+                                if (left >= 8) *reinterpret_cast<uint4*>(to) = make_uint4(v[0], v[1], v[2], v[3]);
+                                if (left >= 16) *reinterpret_cast<uint4*>(to + 8) = make_uint4(v[4], v[5], v[6], v[7]);
+                            } else {
                                 #pragma unroll
-                                for (int z = 0; z < 4; ++z) w[z] = Word<E>::pack(o[e + 2 * z] * f, o[e + 2 * z + 1] * f);
-                                if (task.vector_out) *reinterpret_cast<uint4*>(out + 32 * k + e) = make_uint4(w[0], w[1], w[2], w[3]);
-                                else {
-                                    #pragma unroll
-                                    for (int z = 0; z < 8; ++z) reinterpret_cast<uint16_t*>(out)[32 * k + e + z] = (uint16_t)(w[z >> 1] >> (16 * (z & 1)));
-                                }
+                                for (int z = 0; z < 16; ++z)
+                                    if (z < left) reinterpret_cast<uint16_t*>(to)[z] = (uint16_t)(v[z >> 1] >> (16 * (z & 1)));
                             }
                         }
                     } else {
@@ -588,7 +597,9 @@ int attention_tc_launch(AttnArgs& a, int dtype, bool prefix, cudaStream_t stream
     const int64_t pks[3] = {0, a.pks[0], a.pks[1]}, pvs[3] = {0, a.pvs[0], a.pvs[1]};
     const int64_t *ks = prefix ? pks : a.ks, *vs = prefix ? pvs : a.vs;
     task.k_by_seq = ks[0] > 0; task.k_by_head = ks[1] > 0; task.v_by_seq = vs[0] > 0; task.v_by_head = vs[1] > 0;
-    task.vector_out = ((a.os[0] | a.os[1] | a.os[2]) % 8) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+    const int64_t out_steps = a.os[0] | a.os[1] | a.os[2];
+    const uintptr_t out_at = reinterpret_cast<uintptr_t>(a.out);
+    task.vector_out = (out_steps % 16) == 0 && (out_at & 31) == 0 ? 2 : (out_steps % 8) == 0 && (out_at & 15) == 0 ? 1 : 0;
     CUtensorMap mk, mv;
     const int64_t keys = prefix ? a.P : a.S;
     { const int rc = attention_cache_map(&mk, prefix ? a.pk : a.k, dtype, a.D, TILE, keys, ks[2], a.Hkv, ks[1], a.B, ks[0]); if (rc) return rc; }
