@@ -33,7 +33,7 @@ bool nothing(const hbq_attention* p) { return p->B == 0 || p->L == 0 || p->H == 
 struct Plan {
     bool own_tc, prefix_tc;            // prefix_tc: the prefix has a launch of its own, else it is part of the rows' list
     int prefix, own;                   // the tensor-core kernel's pieces
-    int blocks, shared;                // the few-row kernel's blocks (0: not launched)
+    int blocks, shared, cluster;       // the few-row kernel's blocks (0: not launched)
     int parts;                         // entries of a row's list of parts; 0: every row is written by one block
     int64_t part_bytes, table_bytes, slot_bytes;
     int64_t bytes() const { return part_bytes + table_bytes + slot_bytes; }
@@ -47,7 +47,7 @@ Plan plan_of(const hbq_attention* p)
     c.own_tc = alone && p->L > 1 && p->S > 0;
     if (c.prefix_tc) c.prefix = attention_tc_parts(p, true);
     if (c.own_tc) c.own = attention_tc_parts(p, false);
-    else if (!c.prefix_tc || p->S > 0) c.blocks = attention_rows_blocks(p, !alone, &c.shared);
+    else if (!c.prefix_tc || p->S > 0) c.blocks = attention_rows_blocks(p, !alone, &c.shared, &c.cluster);
     c.parts = c.prefix + c.own + (c.prefix_tc && c.blocks ? 1 : 0);
     if (c.parts == 1) c.parts = 0;
     const auto up = [](int64_t n) { return (n + 31) / 32 * 32; };
@@ -81,7 +81,7 @@ int attention_run(const hbq_attention* p, void* workspace, int64_t workspace_byt
     if (c.blocks < 0) return HBQ_ERR_UNSUPPORTED;
     const int64_t need = c.bytes();
     if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 31))) return HBQ_ERR_WORKSPACE;
-    a.parts = c.parts; a.blocks = c.blocks; a.shared = c.shared;
+    a.parts = c.parts; a.blocks = c.blocks; a.shared = c.shared; a.cluster = c.cluster;
     char* ws = static_cast<char*>(workspace);
     a.part = reinterpret_cast<float*>(ws);
     a.table = reinterpret_cast<int2*>(ws + c.part_bytes);

@@ -18,6 +18,7 @@ struct AttnArgs {
     int parts, part0;
     // The few-row kernel's division of work: `blocks` blocks of equal shares; its table and slots in the workspace.
     int blocks, shared;                                      // shared: shares may begin and end inside a row group
+    int cluster;                                             // else: the blocks of a cluster, which share one group
     int2* table;                                             // of each row group: its first block and how many; 0: undivided
     float* slots;                                            // [blocks][2][16][D] sums, then [blocks][2][16] (maximum, weight)
 };
@@ -60,7 +61,7 @@ __device__ __forceinline__ float2* slot_weight(const AttnArgs& a, int block, int
 // attention_rows.cu
 int attention_rows_launch(const AttnArgs& a, int dtype, cudaStream_t stream);
 int attention_join_launch(const AttnArgs& a, int dtype, cudaStream_t stream);
-int attention_rows_blocks(const hbq_attention* p, bool prefix, int* shared);
+int attention_rows_blocks(const hbq_attention* p, bool prefix, int* shared, int* cluster);
 // attention_tc.cu
 int attention_tc_launch(AttnArgs& a, int dtype, bool prefix, cudaStream_t stream);
 int attention_tc_parts(const hbq_attention* p, bool prefix);

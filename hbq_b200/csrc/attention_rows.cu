@@ -13,6 +13,9 @@
 // The lengths are known on the device alone and may be as different as one key and a hundred thousand.  So the row groups'
 // units of 64 keys form one list over all sequences, of which every block takes an equal share; where a share
 // begins or ends inside a group, its part (sum, maximum, weight) goes to a slot of the block and a second kernel joins.
+// Where no group has many keys and there are few groups, a group belongs to a cluster of up to eight blocks instead, which join
+// their parts through distributed shared memory: one launch, no workspace (one sequence of 1024 keys, 8 key heads: 10.8 -> 7.6 us
+// in a graph).
 #include "attention_dev.cuh"
 #include "tc_dev.cuh"
 
@@ -70,7 +73,8 @@ template <int NK> struct RowsShape {
     static constexpr int STAGE = 2 * TILE;
     static constexpr int RING = RW * STAGES * STAGE;
     static constexpr int JOIN = RW * 16 * (DP + 2) * 4;
-    static constexpr int BYTES = RING > JOIN ? RING : JOIN;
+    static constexpr int BLOCK = 16 * (DP + 2) * 4;          // a cluster: this block's part
+    static constexpr int BYTES = RING > JOIN + BLOCK ? RING : JOIN + BLOCK;
 };
 
 // The maps of a call's cache and prefix.
@@ -80,6 +84,19 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, i
 {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
                  ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void cluster_meet()
+{
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// A float at `addr` of the cluster's block `rank`
+__device__ __forceinline__ float peer_load(uint32_t addr, uint32_t rank)
+{
+    float v;
+    asm volatile("{ .reg .b32 p;\n mapa.shared::cluster.u32 p, %1, %2;\n ld.shared::cluster.f32 %0, [p]; }" : "=f"(v) : "r"(addr), "r"(rank) : "memory");
+    return v;
 }
 
 // The keys of row (b, i) in steps of 16: the prefix's, those of the first `ns` keys, those of keys lo .. p.
@@ -168,9 +185,10 @@ __global__ void __launch_bounds__(RW * 32, BLOCKS_PER_SM) attention_rows_kernel(
         }
         token = low;
     } else {
-        token = blockIdx.x / groups;
+        token = blockIdx.x / a.cluster / groups;
         w0 = 0; w1 = 1;
     }
+    const int rank = a.shared ? 0 : (int)(blockIdx.x % a.cluster), stride = a.shared ? RW : RW * a.cluster;
     const uint32_t ring = smem_u32(smem) + warp * (STAGES * Sh::STAGE), bars = smem_u32(&full[warp * STAGES]);
     uint32_t stage = 0, phase = 0;                                   // the warp's next stage to read, and its parity
     bool ok = given_up == 0;
@@ -191,7 +209,7 @@ __global__ void __launch_bounds__(RW * 32, BLOCKS_PER_SM) attention_rows_kernel(
         slot = take == units ? -1 : off > 0 ? 0 : 1;
         if (off == 0 && threadIdx.x == 0)
             a.table[(int64_t)token * groups + g] = make_int2(blockIdx.x, slot < 0 ? 0 : rows_owner(w0 + units - 1, total, takers) - (int)blockIdx.x + 1);
-    } else g = blockIdx.x - token * groups;
+    } else g = blockIdx.x / a.cluster - token * groups;
     const uint32_t hk = g / tiles, g0 = (g - hk * tiles) * 16, rows = min(16u, a.G - g0), h0 = hk * a.G + g0;
     const int kh = a.ks[1] > 0 ? (int)hk : 0, kb = a.ks[0] > 0 ? (int)b : 0, vh = a.vs[1] > 0 ? (int)hk : 0, vb = a.vs[0] > 0 ? (int)b : 0;
     const int ph = a.pks[0] > 0 ? (int)hk : 0, pvh = a.pvs[0] > 0 ? (int)hk : 0;
@@ -208,11 +226,11 @@ __global__ void __launch_bounds__(RW * 32, BLOCKS_PER_SM) attention_rows_kernel(
             load_box(dst + Sh::TILE + h * (GROUP * 128), pre ? &maps.pv : &maps.v, h * 64, j, pre ? pvh : vh, pre ? 0 : vb, bar);
         }
     };
-    const int first = x0 + warp;
+    const int first = x0 + rank * RW + warp;
     if (lane == 0 && ok) {
         uint32_t st = stage;
-        for (int k = 0; k < STAGES && first + k * RW < x1; ++k) {
-            load(first + k * RW, st);
+        for (int k = 0; k < STAGES && first + k * stride < x1; ++k) {
+            load(first + k * stride, st);
             if (++st == STAGES) st = 0;
         }
     }
@@ -235,7 +253,7 @@ __global__ void __launch_bounds__(RW * 32, BLOCKS_PER_SM) attention_rows_kernel(
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
     const float c = a.scale_log2;
 
-    for (int x = first; x < x1 && ok; x += RW) {
+    for (int x = first; x < x1 && ok; x += stride) {
         {
             uint32_t it = 0;
             while (!__all_sync(0xFFFFFFFFu, mbar_try_wait(bars + 8 * stage, phase)))
@@ -311,9 +329,9 @@ __global__ void __launch_bounds__(RW * 32, BLOCKS_PER_SM) attention_rows_kernel(
             Mma<E>::run(o[2 * t + 1], rest, f[2], f[3]);
         }
         __syncwarp();                                                // every lane has read the stage
-        if (lane == 0 && x + STAGES * RW < x1) {
+        if (lane == 0 && x + STAGES * stride < x1) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            load(x + STAGES * RW, stage);
+            load(x + STAGES * stride, stage);
         }
         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
     }
@@ -322,6 +340,19 @@ __global__ void __launch_bounds__(RW * 32, BLOCKS_PER_SM) attention_rows_kernel(
         l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 1);
         l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 2);
     }
+
+    // a row's value: the output, or its part
+    const auto put = [&](uint32_t row, uint32_t d, float top, float weight, float sum) {
+        if (a.parts > 0) {
+            const int64_t at = ((int64_t)b * a.L + i) * a.H + h0 + row;
+            part_sum(a, at, a.part0)[d] = sum;
+            if (d == 0) *part_weight(a, at, a.part0) = make_float2(top, weight);
+        } else {
+            Mma<E>::store(a.out, (int64_t)b * a.os[0] + (int64_t)i * a.os[1] + (int64_t)(h0 + row) * a.os[2] + d, weight == 0.f ? 0.f : sum / weight);
+        }
+    };
+    float* block = reinterpret_cast<float*>(smem + Sh::JOIN);
+    float* block_w = block + 16 * Sh::DP;
 
     // join the warps: [warp][16][DP] sums, then [warp][16] maxima and weights
     __syncthreads();
@@ -354,13 +385,35 @@ __global__ void __launch_bounds__(RW * 32, BLOCKS_PER_SM) attention_rows_kernel(
         if (slot >= 0) {
             slot_sum(a, blockIdx.x, slot, row)[d] = sum;
             if (d == 0) *slot_weight(a, blockIdx.x, slot, row) = make_float2(top, weight);
-        } else if (a.parts > 0) {
-            const int64_t at = ((int64_t)b * a.L + i) * a.H + h0 + row;
-            part_sum(a, at, a.part0)[d] = sum;
-            if (d == 0) *part_weight(a, at, a.part0) = make_float2(top, weight);
-        } else {
-            Mma<E>::store(a.out, (int64_t)b * a.os[0] + (int64_t)i * a.os[1] + (int64_t)(h0 + row) * a.os[2] + d, weight == 0.f ? 0.f : sum / weight);
+        } else if (!a.shared && a.cluster > 1) {
+            block[row * Sh::DP + d] = sum;
+            if (d == 0) { block_w[row * 2] = top; block_w[row * 2 + 1] = weight; }
+        } else put(row, d, top, weight, sum);
+    }
+    if (!a.shared && a.cluster > 1) {
+        // the cluster's parts: every block takes its share of the outputs and reads all blocks' values of them
+        cluster_meet();
+        for (uint32_t x = rank * RW * 32 + threadIdx.x; x < rows * a.D; x += a.cluster * RW * 32) {
+            const uint32_t row = x / a.D, d = x - row * a.D, at = smem_u32(block + row * Sh::DP + d), wat = smem_u32(block_w + row * 2);
+            float tops[8], weights[8], sums[8], top = -INFINITY, sum = 0.f, weight = 0.f;
+            #pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                tops[k] = -INFINITY; weights[k] = sums[k] = 0.f;
+                if (k < a.cluster) { tops[k] = peer_load(wat, k); weights[k] = peer_load(wat + 4, k); sums[k] = peer_load(at, k); }
+            }
+            #pragma unroll
+            for (int k = 0; k < 8; ++k) if (weights[k] != 0.f) top = fmaxf(top, tops[k]);
+            const float ref = top == -INFINITY ? 0.f : top;
+            #pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if (weights[k] == 0.f) continue;                     // (a NaN is no zero)
+                const float f = exp2_fast(tops[k] - ref);
+                sum = fmaf(sums[k], f, sum);
+                weight = fmaf(weights[k], f, weight);
+            }
+            put(row, d, top, weight, sum);
         }
+        cluster_meet();                                              // (the others still read this block's memory)
     }
     w0 += take;
     if (a.shared && w0 < w1) {
@@ -470,7 +523,8 @@ template <class E, int NK>
 int rows_launch(const AttnArgs& a, const RowsMaps& maps, cudaStream_t stream)
 {
     { const int rc = ensure_dynamic_smem(attention_rows_kernel<E, NK>, RowsShape<NK>::BYTES); if (rc) return rc; }
-    HBQ_CUDA_TRY(launch_dependent(attention_rows_kernel<E, NK>, (unsigned)a.blocks, RW * 32, (size_t)RowsShape<NK>::BYTES, stream, a, maps, (a.G + 15) / 16));
+    const unsigned cluster = a.shared ? 1u : (unsigned)a.cluster;
+    HBQ_CUDA_TRY(launch_dependent_clusters(attention_rows_kernel<E, NK>, (unsigned)a.blocks, cluster, RW * 32, (size_t)RowsShape<NK>::BYTES, stream, a, maps, (a.G + 15) / 16));
     HBQ_LAUNCH_CHECK("attention_rows_kernel");
     return HBQ_OK;
 }
@@ -489,24 +543,25 @@ int rows_type(const AttnArgs& a, const RowsMaps& maps, cudaStream_t stream)
 
 }  // namespace
 
-// Blocks of the few-row kernel; prefix: a row's list begins with it.  Shares of equal size over the blocks that are resident at once; a block a
-// row group where there are too many tokens for the table, or where every group is a unit or two by its bounds alone.
-int attention_rows_blocks(const hbq_attention* p, bool prefix, int* shared)
+// Blocks of the few-row kernel; prefix: a row's list begins with it.  A cluster of up to eight blocks a row group as far as
+// all are resident at once and none has more than 512 keys (8 steps a warp; the join of shares costs as much as 4000 keys
+// spread over eight blocks); else shares of equal size over the blocks that are resident, or a block a group where there are
+// too many tokens for the table.
+int attention_rows_blocks(const hbq_attention* p, bool prefix, int* shared, int* cluster)
 {
     int sms = 148;
     device_sms(&sms);
-    const int64_t groups = p->Hkv * ((p->H / p->Hkv + 15) / 16), tokens = p->B * p->L;
+    const int64_t all = p->Hkv * ((p->H / p->Hkv + 15) / 16) * p->B * p->L, most = BLOCKS_PER_SM * sms;
     int64_t keys = p->S;
     if (p->window > 0 && p->window + p->sinks < keys) keys = p->window + p->sinks;
     if (prefix) keys += p->P;
-    const int64_t units = (keys + RW * GROUP - 1) / (RW * GROUP) + 1;
-    if (tokens > RW * 64 || units <= 2) {
-        *shared = 0;
-        return groups * tokens > 0x7FFFFFFF ? -1 : (int)(groups * tokens);
-    }
-    *shared = 1;
-    const int64_t most = units * groups * tokens;
-    return (int)(most < BLOCKS_PER_SM * sms ? most : BLOCKS_PER_SM * sms);
+    int c = 8;
+    while (c > 1 && (all * c > most || keys <= 64 * (c / 2))) c /= 2;
+    *shared = keys > 512 * c && p->B * p->L <= RW * 64;
+    *cluster = *shared || keys > 512 * c ? 1 : c;
+    if (!*shared) return all > 0x7FFFFFFF / 8 ? -1 : (int)(all * *cluster);
+    const int64_t units = ((keys + RW * GROUP - 1) / (RW * GROUP) + 1) * all;
+    return (int)(units < most ? units : most);
 }
 
 int attention_rows_launch(const AttnArgs& a, int dtype, cudaStream_t stream)
