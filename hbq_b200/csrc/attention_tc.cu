@@ -133,6 +133,9 @@ template <> struct Word<__nv_bfloat16> {
     static __device__ __forceinline__ float up(uint16_t u) { return __uint_as_float((uint32_t)u << 16); }
 };
 
+// The first n bits
+__device__ __forceinline__ uint32_t first_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
+
 // What the rows of a block see, in key positions: all rows that see anything stand between pa and pb.
 struct Span {
     int pa, pb, window, sinks;         // window: 0 for none
@@ -211,7 +214,9 @@ __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_const
             sp.count = sp.first_tiles + sp.pb / TILE - sp.low_tile + 1;
         }
     }
-    const int u0 = (int)((int64_t)sp.count * split / a.nsplit), u1 = (int)((int64_t)sp.count * (split + 1) / a.nsplit), nt = u1 - u0;
+    // (a piece's tiles: counts times pieces stay below 2^31, keys being fewer than 2^31 and pieces 64)
+    const int u0 = a.nsplit == 1 ? 0 : (int)((uint32_t)sp.count * split / (uint32_t)a.nsplit);
+    const int u1 = a.nsplit == 1 ? sp.count : (int)((uint32_t)sp.count * (split + 1) / (uint32_t)a.nsplit), nt = u1 - u0;
 
     if (warp == 9) {
         // ================= keys and values =================
@@ -324,8 +329,10 @@ __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_const
             for (int k = 0; k < PIECES; ++k) {
                 const int row = k * (32 / PIECES) + lane / PIECES, pc = lane % PIECES;
                 const int64_t from = __shfl_sync(0xFFFFFFFFu, at, row);
-                x[k] = make_uint4(0, 0, 0, 0);
-                if (from >= 0 && pc * 8 < (int)a.D) x[k] = *reinterpret_cast<const uint4*>(static_cast<const E*>(a.q) + from + pc * 8);
+                const bool in = from >= 0 && pc * 8 < (int)a.D;    // (else the first row's first values, which are not used: a load
+                                                                   // under a condition would wait for the one before)
+                x[k] = *reinterpret_cast<const uint4*>(static_cast<const E*>(a.q) + (in ? from + pc * 8 : 0));
+                if (!in) x[k] = make_uint4(0, 0, 0, 0);
             }
             #pragma unroll
             for (int k = 0; k < PIECES; ++k) {
@@ -340,6 +347,42 @@ __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_const
         uint32_t vs = 1, vph = 0;                            // ring entry of this step's values
         if (t == 0 || two)
         for (int u = 0; u < nt; ++u) {
+            const int j0 = sp.tile(u0 + u) * TILE;
+            const bool whole = sp.whole(j0);
+            if (!whole && t == 0) {
+                // infinities and NaNs among this tile's values, while the scores are on their way: thread = key
+                if (!(ok = wait_for(kv_full + 8 * vs, vph, abort_flag, 46))) break;
+                const uint32_t row = ring + vs * Sh::STAGE + wr * 128;
+                constexpr uint32_t EXPONENTS = Word<E>::INF * 0x10001u, ONE = (0x8000u - Word<E>::INF) * 0x10001u;
+                bool found = false;
+                #pragma unroll
+                for (int pc = 0; pc < DP / 8; ++pc) {
+                    const uint32_t at = row + (pc >> 3) * (TILE * 128) + (((pc & 7) ^ (wr & 7)) * 16);
+                    uint32_t v[4];
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
+                    uint32_t bad = 0;                        // (an exponent of ones and one more sets the bit above it)
+                    #pragma unroll
+                    for (int e = 0; e < 4; ++e) bad |= (v[e] & EXPONENTS) + ONE;
+                    if (bad & 0x80008000u) found = true;
+                }
+                if (found) {
+                    if (sp.seen_by_some(j0 + wr)) { *special = 1; __threadfence_block(); }
+                    #pragma unroll 1
+                    for (int pc = 0; pc < DP / 8; ++pc) {
+                        const uint32_t at = row + (pc >> 3) * (TILE * 128) + (((pc & 7) ^ (wr & 7)) * 16);
+                        #pragma unroll 1
+                        for (int e = 0; e < 4; ++e) {
+                            uint32_t v;
+                            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at + 4 * e) : "memory");
+                            if ((v & Word<E>::INF) == Word<E>::INF) v &= 0xFFFF0000u;
+                            if ((v & (Word<E>::INF << 16)) == (Word<E>::INF << 16)) v &= 0x0000FFFFu;
+                            asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + 4 * e), "r"(v) : "memory");
+                        }
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
+                __syncwarp();
+            }
             if (!(ok = wait_for(s_full + 8 * t, (uint32_t)u & 1u, abort_flag, 45))) break;
             tc_fence_after();
             uint32_t s[128];
@@ -348,13 +391,15 @@ __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_const
             tc_ld_wait(s);
             #pragma unroll
             for (int k = 1; k < 4; ++k) tc_ld_landed(s + 32 * k);
-            const int j0 = sp.tile(u0 + u) * TILE;
-            const bool whole = sp.whole(j0);
             if (!whole) {
-                const int top = hi - j0, low = lo - j0, sink = sp.sinks - j0;
                 #pragma unroll
-                for (int k = 0; k < 128; ++k)
-                    if (k > top || (k < low && k >= sink)) s[k] = 0xFF800000u;
+                for (int q = 0; q < 4; ++q) {
+                    const int k0 = j0 + 32 * q;
+                    const uint32_t seen = first_bits(hi + 1 - k0) & (~first_bits(lo - k0) | first_bits(sp.sinks - k0));
+                    #pragma unroll
+                    for (int k = 0; k < 32; ++k)
+                        if (!(seen & (1u << k))) s[32 * q + k] = 0xFF800000u;
+                }
             }
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
             #pragma unroll
@@ -396,33 +441,6 @@ __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_const
                     s[32 * q + 2 * k] = __float_as_uint(x); s[32 * q + 2 * k + 1] = __float_as_uint(y);
                 }
                 tc_st16(s_col + 16 * q, w);
-            }
-            if (!whole && t == 0) {
-                // infinities and NaNs among this tile's values: thread = key
-                if (!(ok = wait_for(kv_full + 8 * vs, vph, abort_flag, 46))) break;
-                const uint32_t row = ring + vs * Sh::STAGE + wr * 128;
-                bool found = false;
-                #pragma unroll 4
-                for (int pc = 0; pc < DP / 8; ++pc) {
-                    const uint32_t at = row + (pc >> 3) * (TILE * 128) + (((pc & 7) ^ (wr & 7)) * 16);
-                    uint32_t x[4];
-                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at) : "memory");
-                    constexpr uint32_t LOW = Word<E>::INF, HIGH = Word<E>::INF << 16;
-                    bool bad = false;
-                    #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const bool b0 = (x[e] & LOW) == LOW, b1 = (x[e] & HIGH) == HIGH;
-                        bad |= b0 || b1;
-                        if (b0) x[e] &= 0xFFFF0000u;
-                        if (b1) x[e] &= 0x0000FFFFu;
-                    }
-                    if (bad) {
-                        found = true;
-                        if (sp.seen_by_some(j0 + wr)) { *special = 1; __threadfence_block(); }
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
-                    }
-                }
-                if (found) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             }
             vs += 2;
             if (vs >= Sh::NS) { vs -= Sh::NS; vph ^= 1u; }
