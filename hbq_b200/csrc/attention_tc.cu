@@ -33,9 +33,7 @@ template <int DP> struct TcShape {
 
 struct TcTask {
     uint32_t R;                        // rows of a key head: L * G, or B * L * G against a prefix
-    uint32_t groups;                   // sequences with keys of their own: B, or 1
-    uint32_t tiles;                    // row tiles of 256
-    int prefix, k_by_head, k_by_seq, v_by_head, v_by_seq, vector_out;
+    int prefix, k_by_head, k_by_seq, v_by_head, v_by_seq, vector_out, tma_out;
 };
 
 // Bounded wait of one thread, and of a warp by its lane 0 (a poll by all lanes is 32 accesses to the barrier's word, beside
@@ -67,6 +65,32 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
 {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
                  ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar) : "memory");
+}
+// A warp's 32 rows from shared memory, once every lane has written its own (whole warp)
+__device__ __forceinline__ void rows_written()
+{
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+}
+__device__ __forceinline__ void store_rows(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2, int c3)
+{
+    rows_written();
+    if ((threadIdx.x & 31) == 0)
+        asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];\n cp.async.bulk.commit_group;"
+                     ::"l"(map), "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
+}
+__device__ __forceinline__ void store_parts(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2, int c3, int c4)
+{
+    rows_written();
+    if ((threadIdx.x & 31) == 0)
+        asm volatile("cp.async.bulk.tensor.5d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5, %6}], [%1];\n cp.async.bulk.commit_group;"
+                     ::"l"(map), "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4) : "memory");
+}
+// The stores so far have read their memory (whole warp)
+__device__ __forceinline__ void rows_read()
+{
+    if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncwarp();
 }
 __device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate)
 {
@@ -152,6 +176,7 @@ struct Span {
 
 template <class E, int DP>
 __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                              const __grid_constant__ CUtensorMap map_o,
                                                               const __grid_constant__ AttnArgs a, const __grid_constant__ TcTask task)
 {
     using Sh = TcShape<DP>;
@@ -187,11 +212,8 @@ __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_const
 
     // this block: rows r0 .. r0 + 255 of key head hk of a sequence (group), a piece of their keys; the rows that see the
     // most keys first, so that the last blocks to start are short ones
-    uint32_t id = blockIdx.x;
-    const uint32_t split = id % (uint32_t)a.nsplit; id /= (uint32_t)a.nsplit;
-    const uint32_t hk = id % a.Hkv; id /= a.Hkv;
-    const uint32_t group = id % task.groups;
-    const uint32_t r0 = (task.tiles - 1 - id / task.groups) * 256u, rend = min(r0 + 256u, task.R);
+    const uint32_t hk = blockIdx.x / (uint32_t)a.nsplit, split = blockIdx.x - hk * a.nsplit, group = blockIdx.y;
+    const uint32_t r0 = (gridDim.z - 1 - blockIdx.z) * 256u, rend = min(r0 + 256u, task.R);
     const bool two = r0 + TILE < task.R;
 
     int64_t n64 = 0, first = 0;
@@ -296,14 +318,20 @@ __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_const
     } else {
         // ================= rows =================
         const int t = warp >> 2, wr = (warp & 3) * 32 + lane;
-        const uint32_t r = r0 + t * TILE + wr;
-        uint32_t b = group, i = 0, h = 0;
+        // sequence, token and head of the thread's row; found again for the results, not kept: the loop needs every register
+        const auto row_at = [&](uint32_t r, uint32_t& b, uint32_t& i, uint32_t& h) {
+            asm volatile("" : "+r"(r));
+            b = group;
+            if (task.prefix) { b = r / (a.L * a.G); r -= b * (a.L * a.G); }
+            i = r / a.G;
+            h = hk * a.G + (r - i * a.G);
+        };
         int hi = -1, lo = 0;                                 // this row sees keys lo .. hi and those before sp.sinks
-        if (r < rend) {
-            uint32_t rr = r;
-            if (task.prefix) { b = rr / (a.L * a.G); rr -= b * (a.L * a.G); }
-            i = rr / a.G;
-            h = hk * a.G + (rr - i * a.G);
+        int64_t at = -1;                                     // its queries
+        if (r0 + t * TILE + wr < rend) {
+            uint32_t b, i, h;
+            row_at(r0 + t * TILE + wr, b, i, h);
+            at = (int64_t)b * a.qs[0] + (int64_t)i * a.qs[1] + (int64_t)h * a.qs[2];
             if (task.prefix) sequence_of(a, b, &n64, &first);
             const int64_t p = first + i;
             if (p < n64) {
@@ -315,31 +343,25 @@ __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_const
             }
         }
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        const uint32_t s_col = lanes + t * TILE, o_col = lanes + 2 * TILE + t * DP;
+        const uint32_t s_col = lanes + t * TILE, o_col = s_col + 2 * TILE + t * (DP - TILE);
         bool ok = true;
         float m = -INFINITY, l = 0.f;
         const float c = a.scale_log2;
         if (nt > 0) {
-            // queries of this warp's 32 rows: 16-byte pieces, neighbouring lanes along a row, all loads at once (four at a time
-            // cost a block of few keys 2 us); a row's address comes from the lane that owns the row
+            // queries of this warp's 32 rows: 16-byte pieces, neighbouring lanes along a row, all on their way at once; a row's
+            // address comes from the lane that owns the row.  (Little code, too: what a block runs once it fetches cold.)
             constexpr int PIECES = DP / 8;
-            const int64_t at = r < rend ? (int64_t)b * a.qs[0] + (int64_t)i * a.qs[1] + (int64_t)h * a.qs[2] : -1;
-            uint4 x[PIECES];
-            #pragma unroll
+            const int pc = lane % PIECES, own = lane / PIECES;
+            #pragma unroll 4
             for (int k = 0; k < PIECES; ++k) {
-                const int row = k * (32 / PIECES) + lane / PIECES, pc = lane % PIECES;
-                const int64_t from = __shfl_sync(0xFFFFFFFFu, at, row);
-                const bool in = from >= 0 && pc * 8 < (int)a.D;    // (else the first row's first values, which are not used: a load
-                                                                   // under a condition would wait for the one before)
-                x[k] = *reinterpret_cast<const uint4*>(static_cast<const E*>(a.q) + (in ? from + pc * 8 : 0));
-                if (!in) x[k] = make_uint4(0, 0, 0, 0);
-            }
-            #pragma unroll
-            for (int k = 0; k < PIECES; ++k) {
-                const uint32_t q = warp * 32 + k * (32 / PIECES) + lane / PIECES, pc = lane % PIECES;
+                const int64_t from = __shfl_sync(0xFFFFFFFFu, at, k * (32 / PIECES) + own);
+                const bool in = from >= 0 && pc * 8 < (int)a.D;
+                const E* p = static_cast<const E*>(a.q) + (in ? from + pc * 8 : 0);
+                const uint32_t q = warp * 32 + k * (32 / PIECES) + own;
                 const uint32_t dst = qs + (pc >> 3) * (2 * TILE * 128) + q * 128 + (((pc & 7) ^ (q & 7)) * 16);
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(x[k].x), "r"(x[k].y), "r"(x[k].z), "r"(x[k].w) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(p), "r"(in ? 16 : 0) : "memory");
             }
+            asm volatile("cp.async.wait_all;" ::: "memory");
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full);
@@ -438,19 +460,17 @@ __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_const
                     if ((k & 3) == 3) exp2_pair(x, y);          // a quarter of them
                     else { x = exp2_fast(x); y = exp2_fast(y); }
                     w[k] = Word<E>::pack(x, y);
-                    s[32 * q + 2 * k] = __float_as_uint(x); s[32 * q + 2 * k + 1] = __float_as_uint(y);
+                    add2(sum[2 * (k & 1)], sum[2 * (k & 1) + 1], x, y);
                 }
                 tc_st16(s_col + 16 * q, w);
             }
             vs += 2;
             if (vs >= Sh::NS) { vs -= Sh::NS; vph ^= 1u; }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             tc_st_wait();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(p_ready + 8 * t);
-            #pragma unroll
-            for (int k = 0; k < 64; ++k) add2(sum[2 * (k & 1)], sum[2 * (k & 1) + 1], __uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]));
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         }
         // ---- the rows' results ----
         if (ok && (t == 0 || two)) {
@@ -459,10 +479,21 @@ __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_const
             const bool direct = a.parts == 0, add = nt > 0 && *special;
             const bool live = hi >= 0 && l != 0.f;            // (a NaN counts as something)
             const float f = direct ? (live ? 1.f / l : 0.f) : 1.f;
+            const uint32_t r = r0 + t * TILE + wr;
+            uint32_t b, i, h;
+            row_at(r, b, i, h);
             const int64_t row = ((int64_t)b * a.L + i) * a.H + h;
-            E* out = static_cast<E*>(a.out) + (int64_t)b * a.os[0] + (int64_t)i * a.os[1] + (int64_t)h * a.os[2];
-            float* part = direct ? nullptr : part_sum(a, row, a.part0 + split);
             if (ok) {
+                // Results leave by TMA where the warp's 32 rows are whole tokens (map_o: G heads by 32 / G tokens): each lane puts its
+                // row into this row tile's queries' memory, which no product reads any more.  Stores of a row a lane touch 32 lines at
+                // a time (4000 cycles a block).
+                const uint32_t region = qs + warp * 4096;              // 32 rows of 128 bytes; the next 64 columns' lie 2 * TILE rows on
+                const auto stage_in = [&](uint32_t at, int pc, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + lane * 128 + ((pc ^ (lane & 7)) * 16)), "r"(w0), "r"(w1), "r"(w2), "r"(w3) : "memory");
+                };
+                const uint32_t base_row = r0 + warp * 32;
+                const int token = (int)(base_row / a.G), seq = task.prefix ? 0 : (int)group;
+                const bool by_tma = task.tma_out && base_row < rend;   // (rows behind the last: nothing)
                 #pragma unroll 1
                 for (int k = 0; k < DP / 32; ++k) {
                     float o[32];
@@ -493,29 +524,36 @@ __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_const
                             }
                         }
                     }
-                    if (r >= rend) {
-                    } else if (direct) {
+                    if (direct) {
                         uint32_t w[16];
                         #pragma unroll
                         for (int z = 0; z < 16; ++z) w[z] = Word<E>::pack(o[2 * z] * f, o[2 * z + 1] * f);
-                        #pragma unroll
-                        for (int e = 0; e < 32; e += 16) {
-                            E* to = out + 32 * k + e;
-                            const uint32_t* v = w + e / 2;
-                            const int left = (int)a.D - 32 * k - e;
-                            if (task.vector_out == 2 && left >= 16)  // whole sectors
-                                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]),
-                                             "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
-                            else if (task.vector_out) {
-                                if (left >= 8) *reinterpret_cast<uint4*>(to) = make_uint4(v[0], v[1], v[2], v[3]);
-                                if (left >= 16) *reinterpret_cast<uint4*>(to + 8) = make_uint4(v[4], v[5], v[6], v[7]);
-                            } else {
-                                #pragma unroll
-                                for (int z = 0; z < 16; ++z)
-                                    if (z < left) reinterpret_cast<uint16_t*>(to)[z] = (uint16_t)(v[z >> 1] >> (16 * (z & 1)));
+                        if (by_tma) {
+                            const uint32_t at = region + (k >> 1) * (2 * TILE * 128);
+                            #pragma unroll
+                            for (int e = 0; e < 4; ++e) stage_in(at, 4 * (k & 1) + e, w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+                            if (k & 1) store_rows(&map_o, at, 64 * (k >> 1), (int)(hk * a.G), token, seq);
+                        } else if (r < rend) {
+                            uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (int64_t)b * a.os[0] + (int64_t)i * a.os[1] + (int64_t)h * a.os[2] + 32 * k;
+                            #pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                if (32 * k + 8 * e >= (int)a.D) break;
+                                if (task.vector_out) *reinterpret_cast<uint4*>(out + 8 * e) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+                                else {
+                                    #pragma unroll
+                                    for (int z = 0; z < 8; ++z) out[8 * e + z] = (uint16_t)(w[4 * e + (z >> 1)] >> (16 * (z & 1)));
+                                }
                             }
                         }
-                    } else {
+                    } else if (by_tma) {
+                        const uint32_t at = region + (k & (DP / 64 - 1)) * (2 * TILE * 128);
+                        if (k >= DP / 64 && (k & (DP / 64 - 1)) == 0) rows_read();
+                        #pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            stage_in(at, e, __float_as_uint(o[4 * e]), __float_as_uint(o[4 * e + 1]), __float_as_uint(o[4 * e + 2]), __float_as_uint(o[4 * e + 3]));
+                        store_parts(&map_o, at, 32 * k, a.part0 + (int)split, (int)(hk * a.G), token, seq);
+                    } else if (r < rend) {
+                        float* part = part_sum(a, row, a.part0 + split);
                         #pragma unroll
                         for (int e = 0; e < 32; e += 8)          // whole sectors
                             if (32 * k + e < (int)a.D)
@@ -523,6 +561,7 @@ __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_const
                                              "f"(o[e + 2]), "f"(o[e + 3]), "f"(o[e + 4]), "f"(o[e + 5]), "f"(o[e + 6]), "f"(o[e + 7]) : "memory");
                     }
                 }
+                if (by_tma && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
                 if (!direct && r < rend)
                     *part_weight(a, row, a.part0 + split) = live ? make_float2((m == -INFINITY ? 0.f : m * c) - SHIFT, l) : make_float2(-INFINITY, 0.f);
             }
@@ -557,11 +596,40 @@ EncodeFn encoder()
     return fn;
 }
 
+int encode(CUtensorMap* map, CUtensorMapDataType type, uint32_t rank, const void* ptr, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box)
+{
+    EncodeFn fn = encoder();
+    if (!fn) return HBQ_ERR_CUDA;
+    const cuuint32_t each[5] = {1, 1, 1, 1, 1};
+    const CUresult r = fn(map, type, rank, const_cast<void*>(ptr), dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? HBQ_OK : HBQ_ERR_CUDA;
+}
+// The output [sequence][token][head][D] in boxes of G heads by 32 / G tokens; against a prefix the sequences' tokens are one
+// axis, where their steps allow it.
+int out_map(CUtensorMap* map, const AttnArgs& a, int dtype, bool prefix)
+{
+    if (prefix && a.L > 1 && a.B > 1 && a.os[0] != (int64_t)a.L * a.os[1]) return HBQ_ERR_UNSUPPORTED;
+    const int64_t tokens = prefix ? (int64_t)a.B * a.L : a.L, step = prefix && a.L == 1 ? a.os[0] : a.os[1];
+    const auto bytes = [&](int64_t stride) { return (cuuint64_t)(stride > 0 ? stride : a.D) * 2; };      // (an axis of one element has any step)
+    const cuuint64_t dims[4] = {a.D, a.H, (cuuint64_t)tokens, prefix ? 1u : a.B}, strides[3] = {bytes(a.os[2]), bytes(step), bytes(a.os[0])};
+    const cuuint32_t box[4] = {64, a.G, 32 / a.G, 1};
+    return encode(map, dtype == HBQ_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, a.out, dims, strides, box);
+}
+// The rows' lists of parts [sequence][token][head][part][D], likewise
+int parts_map(CUtensorMap* map, const AttnArgs& a, bool prefix)
+{
+    const cuuint64_t list = (cuuint64_t)a.parts * a.D * 4, token = list * a.H, tokens = prefix ? (cuuint64_t)a.B * a.L : a.L;
+    const cuuint64_t dims[5] = {a.D, (cuuint64_t)a.parts, a.H, tokens, prefix ? 1u : a.B}, strides[4] = {a.D * 4ull, list, token, token * a.L};
+    const cuuint32_t box[5] = {32, 1, a.G, 32 / a.G, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 5, a.part, dims, strides, box);
+}
+
 template <class E, int DP>
-int tc_launch(const CUtensorMap& mk, const CUtensorMap& mv, const AttnArgs& a, const TcTask& task, unsigned blocks, cudaStream_t stream)
+int tc_launch(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mo, const AttnArgs& a, const TcTask& task, dim3 blocks, cudaStream_t stream)
 {
     { const int rc = ensure_dynamic_smem(attention_tc_kernel<E, DP>, TcShape<DP>::BYTES); if (rc) return rc; }
-    HBQ_CUDA_TRY(launch_dependent(attention_tc_kernel<E, DP>, blocks, TCT, (size_t)TcShape<DP>::BYTES, stream, mk, mv, a, task));
+    HBQ_CUDA_TRY(launch_dependent(attention_tc_kernel<E, DP>, blocks, TCT, (size_t)TcShape<DP>::BYTES, stream, mk, mv, mo, a, task));
     HBQ_LAUNCH_CHECK("attention_tc_kernel");
     return HBQ_OK;
 }
@@ -573,16 +641,11 @@ int tc_launch(const CUtensorMap& mk, const CUtensorMap& mv, const AttnArgs& a, c
 int attention_cache_map(CUtensorMap* map, const void* ptr, int dtype, int64_t D, int rows, int64_t keys, int64_t key_stride, int64_t heads, int64_t head_stride,
               int64_t seqs, int64_t seq_stride)
 {
-    EncodeFn fn = encoder();
-    if (!fn) return HBQ_ERR_CUDA;
     const auto step = [](int64_t stride, int64_t other) { return (cuuint64_t)(stride > 0 ? stride : other) * 2; };
     const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)keys, (cuuint64_t)(head_stride > 0 ? heads : 1), (cuuint64_t)(seq_stride > 0 ? seqs : 1)};
     const cuuint64_t strides[3] = {step(key_stride, D), step(head_stride, D), step(seq_stride, D)};
-    const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, each[4] = {1, 1, 1, 1};
-    const CUresult r = fn(map, dtype == HBQ_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr), dims,
-                          strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? HBQ_OK : HBQ_ERR_CUDA;
+    const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1};
+    return encode(map, dtype == HBQ_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, ptr, dims, strides, box);
 }
 
 // Into how many pieces the keys of a block's rows are cut: the count with the shortest longest SM, where a block costs its
@@ -609,24 +672,28 @@ int attention_tc_launch(AttnArgs& a, int dtype, bool prefix, cudaStream_t stream
     TcTask task = {};
     const int64_t R = (int64_t)(prefix ? a.B : 1) * a.L * a.G;
     if (R > 0x7FFFFF00ll) return HBQ_ERR_UNSUPPORTED;
-    task.R = (uint32_t)R; task.groups = prefix ? 1 : a.B; task.tiles = (task.R + 255) / 256; task.prefix = prefix;
-    const int64_t blocks = (int64_t)task.tiles * task.groups * a.Hkv * a.nsplit;
-    if (blocks > 0x7FFFFFFFll) return HBQ_ERR_UNSUPPORTED;
+    task.R = (uint32_t)R; task.prefix = prefix;
+    const uint32_t tiles = (task.R + 255) / 256;
+    if (tiles > 65535) return HBQ_ERR_UNSUPPORTED;                 // (sequences are at most that many by the call's checks)
+    const dim3 blocks(a.Hkv * (unsigned)a.nsplit, prefix ? 1u : a.B, tiles);
     const int64_t pks[3] = {0, a.pks[0], a.pks[1]}, pvs[3] = {0, a.pvs[0], a.pvs[1]};
     const int64_t *ks = prefix ? pks : a.ks, *vs = prefix ? pvs : a.vs;
     task.k_by_seq = ks[0] > 0; task.k_by_head = ks[1] > 0; task.v_by_seq = vs[0] > 0; task.v_by_head = vs[1] > 0;
-    const int64_t out_steps = a.os[0] | a.os[1] | a.os[2];
-    const uintptr_t out_at = reinterpret_cast<uintptr_t>(a.out);
-    task.vector_out = (out_steps % 16) == 0 && (out_at & 31) == 0 ? 2 : (out_steps % 8) == 0 && (out_at & 15) == 0 ? 1 : 0;
-    CUtensorMap mk, mv;
+    task.vector_out = ((a.os[0] | a.os[1] | a.os[2]) % 8) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+    CUtensorMap mk, mv, mo = {};
+    if (32 % a.G == 0) {
+        const int rc = a.parts ? parts_map(&mo, a, prefix) : task.vector_out ? out_map(&mo, a, dtype, prefix) : HBQ_ERR_UNSUPPORTED;
+        if (rc && rc != HBQ_ERR_UNSUPPORTED) return rc;
+        task.tma_out = rc == HBQ_OK;
+    }
     const int64_t keys = prefix ? a.P : a.S;
     { const int rc = attention_cache_map(&mk, prefix ? a.pk : a.k, dtype, a.D, TILE, keys, ks[2], a.Hkv, ks[1], a.B, ks[0]); if (rc) return rc; }
     { const int rc = attention_cache_map(&mv, prefix ? a.pv : a.v, dtype, a.D, TILE, keys, vs[2], a.Hkv, vs[1], a.B, vs[0]); if (rc) return rc; }
     const bool wide = a.D > 64;
     if (dtype == HBQ_DTYPE_F16)
-        return wide ? tc_launch<__half, 128>(mk, mv, a, task, (unsigned)blocks, stream) : tc_launch<__half, 64>(mk, mv, a, task, (unsigned)blocks, stream);
-    return wide ? tc_launch<__nv_bfloat16, 128>(mk, mv, a, task, (unsigned)blocks, stream)
-                : tc_launch<__nv_bfloat16, 64>(mk, mv, a, task, (unsigned)blocks, stream);
+        return wide ? tc_launch<__half, 128>(mk, mv, mo, a, task, blocks, stream) : tc_launch<__half, 64>(mk, mv, mo, a, task, blocks, stream);
+    return wide ? tc_launch<__nv_bfloat16, 128>(mk, mv, mo, a, task, blocks, stream)
+                : tc_launch<__nv_bfloat16, 64>(mk, mv, mo, a, task, blocks, stream);
 }
 
 int attention_rows_status(int* host_out);   // attention_rows.cu: that kernel's own status word
