@@ -34,11 +34,13 @@ import torch.nn as nn
 
 from . import blockquant_ext as ext
 from . import kvcache
+from .attention import window_attention
 from .fused import rmsnorm_quantize, softmax_quantize
 from .ep_moe import ExpertParallelMoE
 from .module import QLinear
 from .ops import FP16AccumMatMul, FP32AccumMatMul
 from .quantizer import _CudaBlockQuantizer, _QBase, calls_only_its_format
+from .rotary import qk_norm_rope, rope_frequencies, rope_rotate
 
 
 @dataclass
@@ -55,6 +57,16 @@ class LlamaArch:
     theta: float = 500000.0
     num_experts: int = 0          # > 0: a sparse mixture-of-experts MLP (Mixtral), experts spread over the ranks
     top_k: int = 2
+    window: int = 0               # > 0: attention sees the last `window` tokens ...
+    sinks: int = 0                # ... and the first `sinks`
+    qk_norm: bool = False         # an RMS norm of every query and key head in front of the rotation
+    rotary_dim: int = 0           # the values of a head that turn, the first ones; 0: all
+    rope_interleaved: bool = False
+    rope_scaling: Optional[dict] = None     # rope_frequencies' scaling
+
+    def tables(self) -> bool:
+        """The rotation is the one that ``rope_tables`` holds: whole heads, half layout, plain frequencies, no norm before it."""
+        return not (self.qk_norm or self.rope_interleaved or self.rope_scaling) and self.rotary_dim in (0, self.head_dim)
 
 
 def mixtral_8x7b() -> "LlamaArch":
@@ -120,12 +132,47 @@ class QLlamaAttention(nn.Module):
         self.kv_quantizer = None
         self.attn_wgt_quantizer = None
         self.query_chunk = 512                                 # queries per run of a causal prefill (multiple of 128)
+        self.window, self.sinks = arch.window, arch.sinks
+        self.rotary = None                                     # (inv_freq, factor) where the rotation is not the tables'
+        self.q_norm = self.k_norm = None
+        if not arch.tables():
+            self.rotary = rope_frequencies(arch.rotary_dim or D, arch.theta, arch.rope_scaling, device)
+            self.interleaved, self.eps = arch.rope_interleaved, arch.eps
+            if arch.qk_norm:
+                self.q_norm, self.k_norm = (nn.Parameter(torch.ones(D, dtype=torch.float16, device=device)) for _ in range(2))
 
     def input_quantizer(self):
         """The one quantizer that serves q/k/v_proj's input when the three agree (every shipped HBQ configuration;
         MX formats with ``qk_mx_round`` round q/k differently from v), else None."""
         a = self.q_proj.aq
         return a if _same_format(a, self.k_proj.aq) and _same_format(a, self.v_proj.aq) else None
+
+    def _turned(self, q: torch.Tensor, k: torch.Tensor, q_len: int):
+        """Queries and keys ``[B, T, H, D]`` behind their norm and a rotation that the tables do not hold."""
+        freq, factor = self.rotary
+        if freq.device != q.device:
+            self.rotary = (freq := freq.to(q.device)), factor
+        pos = torch.arange(q_len, device=q.device)
+        if self.q_norm is not None:
+            return qk_norm_rope(q, k, self.q_norm, self.k_norm, self.eps, freq, pos, self.interleaved, factor)
+        return tuple(rope_rotate(t, freq, pos, self.interleaved, factor) for t in (q, k))
+
+    def _windowed(self, Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor) -> torch.Tensor:
+        """Causal attention, of a window and the first tokens where there is one, on ``[B, H, T, D]``, as o_proj's rows.  Where the probabilities are
+        quantised, or heads are longer than the one-pass kernel's, it is ``softmax_quantize``'s with the mask in memory."""
+        B, H, T, D = Q.shape
+        aq = self.attn_wgt_quantizer if self.quant_attn_wgt else None
+        if aq is None and D % 8 == 0 and D <= 128:
+            return window_attention(Q.transpose(1, 2), K, V, window=self.window, sinks=self.sinks).view(B * T, H * D)
+        j = torch.arange(T, device=Q.device)
+        hidden = j[None] > j[:, None]
+        if self.window > 0:
+            hidden = hidden | ((j[None] <= j[:, None] - self.window) & (j[None] >= self.sinks))
+        mask = torch.zeros((1, 1, T, T), dtype=Q.dtype, device=Q.device).masked_fill_(hidden, float("-inf"))
+        scores = torch.matmul(Q.reshape(B, K.shape[1], -1, D), K.transpose(-1, -2))
+        P = softmax_quantize(scores.view(B, H, T, T), 1.0 / math.sqrt(D), aq, mask=mask)
+        O = torch.matmul(P.view(scores.shape), V).view(B, H, T, D)
+        return O.transpose(1, 2).reshape(B * T, H * D)
 
     def forward(self, x: torch.Tensor, bsz: int, q_len: int, cos: torch.Tensor, sin: torch.Tensor,
                 input_quantized: bool = False) -> torch.Tensor:
@@ -137,8 +184,11 @@ class QLlamaAttention(nn.Module):
         v = project(self.v_proj, x, input_quantized).view(bsz, q_len, Hkv * D)
         # RoPE, then the post-RoPE Q / K quantizers (src/module.py:158-162), in the cache layout [B, H, T, D] -- the
         # queries of a prefill that runs in pieces (below) piece by piece
+        if self.rotary is not None:
+            q, k = (t.view(bsz, q_len, -1) for t in self._turned(q.view(bsz, q_len, H, D), k.view(bsz, q_len, Hkv, D), q_len))
+            cos = sin = None
         c = self.query_chunk
-        in_runs = q_len > c and q_len % c == 0 and c % 128 == 0
+        in_runs = q_len > c and q_len % c == 0 and c % 128 == 0 and cos is not None and self.window == 0
         Q = Qr = None
         if in_runs and self.quant_post_rope_q and calls_only_its_format(self.q_proj.aq):
             Qr = kvcache.quantize_q_runs(q, H, G, c, self.q_proj.aq, cos, sin)
@@ -147,18 +197,20 @@ class QLlamaAttention(nn.Module):
         elif self.quant_post_rope_q and isinstance(self.q_proj.aq, _CudaBlockQuantizer):
             Q = kvcache.write_k_cache(q, H, self.q_proj.aq, cos, sin)
         else:
-            Q = kvcache.rope_heads(q, H, cos, sin)
+            Q = kvcache.rope_heads(q, H, cos, sin) if cos is not None else q.view(bsz, q_len, H, D).transpose(1, 2)
             if self.quant_post_rope_q:
                 Q = self.q_proj.aq.q(Q)
         if self.quant_k_cache and isinstance(self.kv_quantizer, _CudaBlockQuantizer):
             K = kvcache.write_k_cache(k, Hkv, self.kv_quantizer, cos, sin)
         else:
-            K = kvcache.rope_heads(k, Hkv, cos, sin)
+            K = kvcache.rope_heads(k, Hkv, cos, sin) if cos is not None else k.view(bsz, q_len, Hkv, D).transpose(1, 2)
         # V quantised along the token axis (src/module.py:163-168)
         if self.quant_v_cache and isinstance(self.kv_quantizer, _CudaBlockQuantizer):
             V = kvcache.write_v_cache(v, Hkv, self.kv_quantizer)
         else:
             V = v.view(bsz, q_len, Hkv, D).transpose(1, 2)
+        if self.window > 0 or (self.rotary is not None and not self.quant_attn_wgt):
+            return project(self.o_proj, self._windowed(Q, K, V))
         # repeat_kv without the copy: the G query heads of a key-value head become rows of one matmul.  A causal
         # prefill is cut into runs of `query_chunk` queries, run c against keys [0, end of run c) only: the keys
         # beyond are masked for every query of the run, their probabilities are zeros and whole quantisation blocks
