@@ -91,6 +91,7 @@ int attention_run(const hbq_attention* p, void* workspace, int64_t workspace_byt
         { const int rc = attention_tc_launch(a, p->dtype, true, stream); if (rc) return rc; }
         a.P = 0;
         a.part0 = c.prefix;
+        a.beside = 1;
     }
     if (c.own_tc) {
         a.nsplit = c.own;

@@ -19,6 +19,7 @@ struct AttnArgs {
     // The few-row kernel's division of work: `blocks` blocks of equal shares; its table and slots in the workspace.
     int blocks, shared;                                      // shared: shares may begin and end inside a row group
     int cluster;                                             // else: the blocks of a cluster, which share one group
+    int beside;                                              // second kernel of a call: runs beside the first (begin_beside)
     int2* table;                                             // of each row group: its first block and how many; 0: undivided
     float* slots;                                            // [blocks][2][16][D] sums, then [blocks][2][16] (maximum, weight)
 };
@@ -26,10 +27,10 @@ struct AttnArgs {
 // Rows of sequence b: its keys, and the position of its first row.
 __device__ __forceinline__ void sequence_of(const AttnArgs& a, uint32_t b, int64_t* n, int64_t* first)
 {
-    int64_t len = a.lengths ? (int64_t)a.lengths[b] : a.S;
+    int64_t len = a.lengths ? (int64_t)__ldcg(a.lengths + b) : a.S;
     len = len < 0 ? 0 : len > a.S ? a.S : len;
     *n = len;
-    *first = a.starts ? (int64_t)a.starts[b] : len - (int64_t)a.L;
+    *first = a.starts ? (int64_t)__ldcg(a.starts + b) : len - (int64_t)a.L;
 }
 
 __device__ __forceinline__ float exp2_fast(float x)
@@ -37,6 +38,18 @@ __device__ __forceinline__ float exp2_fast(float x)
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// The second of a call's two attention kernels reads nothing that the first writes, and the first lets it start only behind its
+// own wait, when all before it is complete: it need not wait for the first, and fills the SMs that the first leaves.  It
+// waits at its end instead (its inputs come from L2, past what an SM's cache may hold of them from before), so that the kernel behind it, which joins both kernels' parts, finds both complete.
+__device__ __forceinline__ void begin_beside(const AttnArgs& a)
+{
+    if (!a.beside) { grid_dependency_wait(); dependents_may_start(); }
+}
+__device__ __forceinline__ void end_beside(const AttnArgs& a)
+{
+    if (a.beside) { grid_dependency_wait(); dependents_may_start(); }
 }
 
 // A part's sums and (maximum, weight) of a row; rows are numbered (b * L + i) * H + h.

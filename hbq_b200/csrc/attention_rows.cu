@@ -167,8 +167,7 @@ __global__ void __launch_bounds__(RW * 32, BLOCKS_PER_SM) attention_rows_kernel(
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
-    grid_dependency_wait();
-    dependents_may_start();
+    begin_beside(a);
     const uint32_t groups = a.Hkv * tiles, tokens = a.B * a.L;       // row groups of a token
     int64_t w0, w1, total = 1, takers = 1;                           // this block's share of the units
     uint32_t token;
@@ -176,7 +175,7 @@ __global__ void __launch_bounds__(RW * 32, BLOCKS_PER_SM) attention_rows_kernel(
         count_units(a, table);
         total = table[tokens] * groups;
         takers = rows_takers(a, total);
-        if (blockIdx.x >= takers) return;
+        if (blockIdx.x >= takers) { end_beside(a); return; }
         w0 = total * blockIdx.x / takers; w1 = total * (blockIdx.x + 1) / takers;
         uint32_t low = 0, high = tokens;                             // the last token that begins at or before w0
         while (high - low > 1) {
@@ -243,7 +242,7 @@ __global__ void __launch_bounds__(RW * 32, BLOCKS_PER_SM) attention_rows_kernel(
         for (int f = 0; f < 4; ++f) {
             const uint32_t r = lane / 4 + 8 * (f & 1), d = kk * 16 + (lane & 3) * 2 + 8 * (f >> 1);
             qf[kk][f] = r < rows && d < a.D
-                ? *reinterpret_cast<const uint32_t*>(static_cast<const E*>(a.q) + (int64_t)b * a.qs[0] + (int64_t)i * a.qs[1] + (int64_t)(h0 + r) * a.qs[2] + d) : 0u;
+                ? __ldcg(reinterpret_cast<const unsigned*>(static_cast<const E*>(a.q) + (int64_t)b * a.qs[0] + (int64_t)i * a.qs[1] + (int64_t)(h0 + r) * a.qs[2] + d)) : 0u;
         }
     float o[NK * 2][4];
     #pragma unroll
@@ -429,6 +428,7 @@ __global__ void __launch_bounds__(RW * 32, BLOCKS_PER_SM) attention_rows_kernel(
         while (gtime_ns() - t0 < 200000ull) { }
         __syncthreads();
     }
+    end_beside(a);
 }
 
 // W warps join a row's parts: the tensor-core kernel's, and the few-row kernel's part or slots.  Maxima, then weights and

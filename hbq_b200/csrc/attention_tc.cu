@@ -206,8 +206,7 @@ __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_const
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    grid_dependency_wait();
-    dependents_may_start();
+    begin_beside(a);
     const uint32_t tmem = *tmem_slot;
 
     // this block: rows r0 .. r0 + 255 of key head hk of a sequence (group), a piece of their keys; the rows that see the
@@ -581,6 +580,7 @@ __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_const
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
+    end_beside(a);
 }
 
 typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
