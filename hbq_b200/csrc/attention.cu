@@ -59,16 +59,28 @@ Plan plan_of(const hbq_attention* p)
     return c;
 }
 
-}  // namespace
-
-int64_t attention_workspace_bytes(const hbq_attention* p)
+// Windows and first tokens beyond the cache mean the whole of it (and their sums stay far from 64 bits' end).
+hbq_attention bounded(const hbq_attention* p)
 {
-    return check(p) || nothing(p) ? 0 : plan_of(p).bytes();
+    hbq_attention c = *p;
+    if (c.window >= c.S || c.window < 0) c.window = 0;
+    if (c.sinks > c.S) c.sinks = c.S;
+    return c;
 }
 
-int attention_run(const hbq_attention* p, void* workspace, int64_t workspace_bytes, cudaStream_t stream)
+}  // namespace
+
+int64_t attention_workspace_bytes(const hbq_attention* call)
 {
-    { const int rc = check(p); if (rc || nothing(p)) return rc; }
+    if (check(call) || nothing(call)) return 0;
+    const hbq_attention c = bounded(call);
+    return plan_of(&c).bytes();
+}
+
+int attention_run(const hbq_attention* call, void* workspace, int64_t workspace_bytes, cudaStream_t stream)
+{
+    { const int rc = check(call); if (rc || nothing(call)) return rc; }
+    const hbq_attention bound = bounded(call), *p = &bound;
     AttnArgs a = {};
     a.q = p->q; a.k = p->k; a.v = p->v; a.out = p->out; a.pk = p->prefix_k; a.pv = p->prefix_v;
     a.lengths = p->lengths; a.starts = p->starts;

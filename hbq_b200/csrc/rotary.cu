@@ -270,7 +270,7 @@ int launch_lanes(RotaryArgs& a, int sms, cudaStream_t stream)
     const uint32_t groups = (a.heads0 + PER - 1) / PER + (a.heads - a.heads0 + PER - 1) / PER;
     a.many = a.tokens >= (int64_t)sms * 16;
     const int64_t blocks = a.many ? (a.tokens + WARPS - 1) / WARPS : a.tokens;
-    const unsigned split = a.many ? 1u : (groups + WARPS - 1) / WARPS;
+    const unsigned spread = (groups + WARPS - 1) / WARPS, split = a.many ? 1u : spread < 65535u ? spread : 65535u;
     HBQ_CUDA_TRY(launch_dependent(rotary_kernel<E, LANES, NORM>, dim3((unsigned)blocks, split), WARPS * 32, 0, stream, a));
     HBQ_LAUNCH_CHECK("rotary_kernel");
     return HBQ_OK;

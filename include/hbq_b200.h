@@ -235,7 +235,7 @@ int hbq_gemm_kn_noalloc(const void* A, const void* B, void* C, int64_t M, int64_
 
 /* The tensor-core kernel bounds every wait on an mbarrier.  If one expires the kernel stops,
  * frees its tensor memory and records which wait gave up in a device status word; the output
- * of that call is then undefined.  hbq_gemm_status copies the word to the host (it
+ * of that call is then undefined (the attention kernels' waits likewise).  hbq_gemm_status copies the word to the host (it
  * synchronises the device); 0 = no wait has expired since the last reset.
  * No reference counterpart (the reference kernels do not wait on anything). */
 int hbq_gemm_status(int* status_host);

@@ -240,6 +240,56 @@ def test_of_nothing():
         assert got.shape == (2, L, 4, 64) and not bool(got.any())
 
 
+@pytest.mark.parametrize("H,Hkv", [(64, 1), (96, 2), (40, 1)])
+def test_many_heads_of_one_key_head(H, Hkv):
+    import hbq_b200 as h
+    for L, S in ((1, 700), (1, 40), (9, 300)):
+        q, k, v = _inputs(2, L, H, Hkv, S, 64, torch.bfloat16, 8)
+        lengths = _lengths([S, S - 7])
+        got = h.window_attention(q, k, v, window=200, sinks=2, lengths=lengths)
+        _close(got, *_reference(q, k, v, lengths, None, 200, 2, 1 / 8))
+        pk, pv = (torch.randn((Hkv, 150, 64), device="cuda").bfloat16() for _ in range(2))
+        got = h.shared_prefix_attention(q, pk, pv, k, v, lengths=lengths)
+        _close(got, *_reference(q, k, v, lengths, None, 0, 0, 1 / 8, (pk, pv)))
+
+
+@pytest.mark.parametrize("B,L,H,Hkv", [(1, 3, 2, 2), (2, 4, 4, 4), (1, 15, 1, 1), (1, 17, 1, 1)])
+def test_few_tokens_behind_a_prefix(B, L, H, Hkv):
+    import hbq_b200 as h
+    q, k, v = _inputs(B, L, H, Hkv, 30, 64, torch.float16, 8)
+    pk, pv = (torch.randn((Hkv, 77, 64), device="cuda").half() for _ in range(2))
+    for lengths, starts in ((None, None), (_lengths([25, 2][:B]), None), (_lengths([25, 2][:B]), _lengths([0, 1][:B]))):
+        got = h.shared_prefix_attention(q, pk, pv, k, v, lengths=lengths, starts=starts)
+        _close(got, *_reference(q, k, v, _all(30, B) if lengths is None else lengths, starts, 0, 0, 1 / 8, (pk, pv)))
+
+
+@pytest.mark.parametrize("H", [4, 6])
+@pytest.mark.parametrize("step", [1, 2, 4, 8])
+def test_outputs_of_any_alignment(step, H):
+    """Rows of the output that are not 16 bytes apart, and outputs that begin off a 16-byte boundary."""
+    import hbq_b200 as h
+    for L in (1, 40):
+        q, k, v = _inputs(2, L, H, 2, 90, 64, torch.float16, 3)
+        want = h.window_attention(q, k, v)
+        wide = torch.full((2, L, H, 64 + step), 9.0, device="cuda").half()
+        h.window_attention(q, k, v, out=wide[..., :64])
+        assert torch.equal(wide[..., :64], want) and bool((wide[..., 64:] == 9).all())
+        wide.fill_(9.0)
+        h.window_attention(q, k, v, out=wide[..., step:])
+        assert torch.equal(wide[..., step:], want) and bool((wide[..., :step] == 9).all())
+
+
+def test_windows_and_first_tokens_beyond_the_cache():
+    """The same keys by another division of the work: each result is off by half a step (2^-12) of itself and of its weighted sum
+    of |v|, which is below 3 here -- 2 * 2^-12 * 3 < 2^-9 between them."""
+    import hbq_b200 as h
+    for L in (1, 50):
+        q, k, v = _inputs(2, L, 8, 2, 90, 64, torch.float16, 3)
+        want = h.window_attention(q, k, v)
+        for window, sinks in ((90, 0), (2 ** 40, 5), (2 ** 62, 2 ** 62), (1, 90), (1, 2 ** 62)):
+            _close(h.window_attention(q, k, v, window=window, sinks=sinks), want.double(), 2.0 ** -10 * want.double().abs() + 2.0 ** -9)
+
+
 @pytest.mark.parametrize("L", [1, 90])
 def test_streams_graphs_and_two_calls_at_once(L):
     import hbq_b200 as h
@@ -319,3 +369,39 @@ def test_projection_to_output_with_a_growing_cache(dtype):
         if t0 >= n:                                                       # sequence 0's first tokens as the prefix of a batch of one
             got = h.shared_prefix_attention(qs[:1], kc[0, :, :n], vc[0, :, :n], kc[:1, :, n:], vc[:1, :, n:], lengths=_all(t1 - n, 1))
             _close(got, full[:1, t0:t1], ftol[:1, t0:t1])
+
+
+@pytest.mark.parametrize("L", [1, 40])
+def test_a_chain_that_changes_its_inputs_in_place(L):
+    """Calls one after the other without a synchronisation, each on inputs that were written just before: kernels that start under
+    the one before them see all of it and leave what it still reads."""
+    import hbq_b200 as h
+    D = 128
+    for wait in (True, False):
+        g = torch.Generator(device="cuda").manual_seed(4)
+        q, k, v = _inputs(8, L, 8, 2, 600, D, torch.float16, 3)
+        pk, pv = (torch.randn((2, 500, D), device="cuda", generator=g).half() for _ in range(2))
+        f, _ = h.rope_frequencies(D, 10000.0, device="cuda")
+        w, lengths, pos = torch.ones(D, device="cuda").half(), _all(600, 8), torch.arange(L, device="cuda")
+        steps = []
+        for n in range(6):
+            o = h.shared_prefix_attention(q, pk, pv, k, v, lengths=lengths)
+            q2, k2 = h.qk_norm_rope(o, k[:, :, :L].transpose(1, 2), w, w, 1e-5, f, pos)
+            k[:, :, 100:100 + L] = k2.transpose(1, 2)
+            v[:, :, 7 + n] = o[:, 0, :2]
+            lengths.sub_(17)
+            h.rope_rotate(q2, f, pos, out=q)
+            pv[:, :L] = o[0].transpose(0, 1)[:2]
+            steps += [o, h.window_attention(q, k, v, window=150 + n, sinks=9, lengths=lengths), q.clone()]
+            if wait:
+                torch.cuda.synchronize()
+        if wait:
+            want = steps
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(steps, want))
+
+
+def test_no_wait_ran_out():
+    import hbq_b200 as h
+    torch.cuda.synchronize()
+    assert h.gemm_status() == 0

@@ -149,6 +149,15 @@ def test_special_values_stay_in_their_head():
     assert bool(torch.isfinite(q[clean]).all()) and bool(torch.isnan(q[1, 1]).all()) and bool(torch.isfinite(k[[0, 1, 3]]).all())
 
 
+def test_very_many_heads():
+    """More groups of heads than a grid's second axis holds."""
+    import hbq_b200 as H
+    x = torch.randn((2, 600001, 16), device="cuda").half()
+    f, _ = H.rope_frequencies(16, 10000.0, device="cuda")
+    pos = torch.tensor([3, 70], device="cuda")
+    _close(H.rope_rotate(x, f, pos)[None], *_turned(x.double()[None], f, pos[None], False, 1.0))
+
+
 @pytest.mark.parametrize("shape", [(0, 5, 2, 64), (2, 0, 2, 64), (2, 5, 0, 64)])
 def test_of_nothing(shape):
     import hbq_b200 as H
