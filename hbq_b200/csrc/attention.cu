@@ -28,8 +28,14 @@ int check(const hbq_attention* p)
 
 bool nothing(const hbq_attention* p) { return p->B == 0 || p->L == 0 || p->H == 0; }
 
-// Which kernels a call takes: rows of one token by the warp-level MMA, more rows by the tensor core; the prefix by itself
-// where its rows (of all sequences) are more than the warp-level MMA's 16.
+// Which kernels a call takes.  The few-row kernel, on the warp-level MMA, reads a token's keys for that token alone; the
+// tensor-core kernel reads them once for 256 rows, but takes 7 us and more whatever it does.
+//  * One token a sequence: the few-row kernel.  More tokens: the tensor-core kernel, unless all row groups are resident in the
+//    few-row kernel at once with few keys each ("small" there).  us, few-row and tensor-core, 32 / 8 heads of 128:
+//    1 x 4 tokens of 2048 keys 12.5 and 15.6, 1 x 16 30 and 16, 8 x 2 of 8192 97 and 64, 32 x 2 of 1024 50 and 39.
+//  * A prefix: the tensor-core kernel for all sequences at once and a kernel for their own keys, unless the call is small, or there
+//    is one token to share it: then the prefix is the beginning of the few-row kernel's lists.  us, in the lists and by itself: prefix of
+//    1024, 4 sequences 10.5 and 24, 8 12 and 19, 16 23 and 19; of 16384, 2 sequences 27.5 and 29, 4 39 and 31.
 struct Plan {
     bool own_tc, prefix_tc;            // prefix_tc: the prefix has a launch of its own, else it is part of the rows' list
     int prefix, own;                   // the tensor-core kernel's pieces
@@ -42,12 +48,17 @@ struct Plan {
 Plan plan_of(const hbq_attention* p)
 {
     Plan c = {};
-    c.prefix_tc = p->P > 0 && p->B * p->L * (p->H / p->Hkv) > 16;
-    const bool alone = p->P == 0 || c.prefix_tc;
-    c.own_tc = alone && p->L > 1 && p->S > 0;
+    bool small;
+    const int together = attention_rows_blocks(p, true, &c.shared, &c.cluster, &small);
+    c.prefix_tc = p->P > 0 && !small && p->B * p->L > 1;
+    if (p->P > 0 && !c.prefix_tc) c.blocks = together;
+    else if (p->S > 0 || !c.prefix_tc) {
+        c.blocks = attention_rows_blocks(p, false, &c.shared, &c.cluster, &small);
+        c.own_tc = p->L > 1 && p->S > 0 && !small;
+    }
+    if (c.own_tc || (c.prefix_tc && p->S == 0)) c.blocks = c.shared = 0;
     if (c.prefix_tc) c.prefix = attention_tc_parts(p, true);
     if (c.own_tc) c.own = attention_tc_parts(p, false);
-    else if (!c.prefix_tc || p->S > 0) c.blocks = attention_rows_blocks(p, !alone, &c.shared, &c.cluster);
     c.parts = c.prefix + c.own + (c.prefix_tc && c.blocks ? 1 : 0);
     if (c.parts == 1) c.parts = 0;
     const auto up = [](int64_t n) { return (n + 31) / 32 * 32; };

@@ -74,7 +74,7 @@ __device__ __forceinline__ float2* slot_weight(const AttnArgs& a, int block, int
 // attention_rows.cu
 int attention_rows_launch(const AttnArgs& a, int dtype, cudaStream_t stream);
 int attention_join_launch(const AttnArgs& a, int dtype, cudaStream_t stream);
-int attention_rows_blocks(const hbq_attention* p, bool prefix, int* shared, int* cluster);
+int attention_rows_blocks(const hbq_attention* p, bool prefix, int* shared, int* cluster, bool* small);
 // attention_tc.cu
 int attention_tc_launch(AttnArgs& a, int dtype, bool prefix, cudaStream_t stream);
 int attention_tc_parts(const hbq_attention* p, bool prefix);

@@ -512,7 +512,7 @@ int join_launch(const AttnArgs& a, cudaStream_t stream)
     const int64_t rows = (int64_t)a.B * a.L * a.H;
     if (rows > 0x7FFFFFFFll) return HBQ_ERR_UNSUPPORTED;
     const uint32_t tiles = (a.G + 15) / 16;
-    // (64 x 32 rows of a few parts each, and fewer, are less than the SMs hold at once)
+    // (64 x 32 rows: four warps a row 81 us, one 88, of the whole call; 33536 rows: 175 and 152)
     if (rows <= 4096) HBQ_CUDA_TRY(launch_dependent(attention_join_kernel<E, 4>, (unsigned)rows, 128, 0, stream, a, tiles));
     else HBQ_CUDA_TRY(launch_dependent(attention_join_kernel<E, 1>, (unsigned)((rows + 3) / 4), 128, 0, stream, a, tiles));
     HBQ_LAUNCH_CHECK("attention_join_kernel");
@@ -544,10 +544,11 @@ int rows_type(const AttnArgs& a, const RowsMaps& maps, cudaStream_t stream)
 }  // namespace
 
 // Blocks of the few-row kernel; prefix: a row's list begins with it.  A cluster of up to eight blocks a row group as far as
-// all are resident at once and none has more than 512 keys (8 steps a warp; the join of shares costs as much as 4000 keys
-// spread over eight blocks); else shares of equal size over the blocks that are resident, or a block a group where there are
-// too many tokens for the table.
-int attention_rows_blocks(const hbq_attention* p, bool prefix, int* shared, int* cluster)
+// all are resident at once and none has more than 512 keys (8 steps a warp); else shares of equal size over the blocks that are
+// resident, or a block a group where there are too many tokens for the table.  us, 32 / 8 heads of 128, clusters and shares:
+// one sequence of 512 keys 8.9 and 9.2, 4096 12.2 and 16.7, 8192 18 and 19, 16384 30 and 22; 8 of 2048 14.9 and 22; 64 of 512
+// (a block each) 31 and 37.  `*small`: all row groups are resident and have no more keys than that.
+int attention_rows_blocks(const hbq_attention* p, bool prefix, int* shared, int* cluster, bool* small)
 {
     int sms = 148;
     device_sms(&sms);
@@ -557,6 +558,7 @@ int attention_rows_blocks(const hbq_attention* p, bool prefix, int* shared, int*
     if (prefix) keys += p->P;
     int c = 8;
     while (c > 1 && (all * c > most || keys <= 64 * (c / 2))) c /= 2;
+    *small = all <= most && keys <= 512 * c;
     *shared = keys > 512 * c && p->B * p->L <= RW * 64;
     *cluster = *shared || keys > 512 * c ? 1 : c;
     if (!*shared) return all > 0x7FFFFFFF / 8 ? -1 : (int)(all * *cluster);

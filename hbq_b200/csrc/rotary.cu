@@ -268,7 +268,8 @@ int launch_lanes(RotaryArgs& a, int sms, cudaStream_t stream)
 {
     constexpr int PER = 32 / LANES;
     const uint32_t groups = (a.heads0 + PER - 1) / PER + (a.heads - a.heads0 + PER - 1) / PER;
-    a.many = a.tokens >= (int64_t)sms * 16;
+    // (600 tokens of 32 heads: a warp a token 4.5 us, heads spread 4.9; 1200: 5.5 and 7.0; 300: 3.5 either way)
+    a.many = a.tokens >= (int64_t)sms * 4;
     const int64_t blocks = a.many ? (a.tokens + WARPS - 1) / WARPS : a.tokens;
     const unsigned spread = (groups + WARPS - 1) / WARPS, split = a.many ? 1u : spread < 65535u ? spread : 65535u;
     HBQ_CUDA_TRY(launch_dependent(rotary_kernel<E, LANES, NORM>, dim3((unsigned)blocks, split), WARPS * 32, 0, stream, a));

@@ -83,7 +83,7 @@ def test_one_token(B, H, Hkv, S, D, window, sinks, dtype):
 
 PROMPT = [(1, 2, 1, 1, 2, 64), (1, 16, 4, 1, 16, 128), (2, 100, 4, 2, 100, 64), (1, 257, 8, 2, 257, 128), (3, 65, 6, 2, 130, 80), (1, 300, 7, 1, 1000, 128),
           (2, 33, 40, 2, 33, 64), (1, 1000, 2, 2, 1000, 96), (1, 513, 5, 1, 2000, 64), (2, 3, 32, 8, 700, 128), (1, 64, 3, 3, 64, 8), (1, 129, 16, 16, 129, 112),
-          (1, 8, 20, 1, 5000, 128)]
+          (1, 8, 20, 1, 5000, 128), (4, 90, 40, 2, 90, 64), (2, 150, 5, 1, 180, 72), (20, 16, 4, 1, 16, 128), (9, 33, 24, 3, 40, 128), (3, 100, 6, 6, 260, 8)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
@@ -123,7 +123,7 @@ def test_lengths_and_starts(L, S, window, sinks, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-@pytest.mark.parametrize("L,S,window,sinks", [(40, 200, 0, 0), (300, 300, 0, 0), (300, 700, 90, 2), (1, 300, 30, 2), (2, 5, 0, 0)])
+@pytest.mark.parametrize("L,S,window,sinks", [(40, 200, 0, 0), (300, 300, 0, 0), (300, 700, 90, 2), (1, 300, 30, 2), (2, 5, 0, 0), (149, 260, 0, 0), (149, 400, 60, 2), (200, 200, 5, 130)])
 def test_what_a_mask_hides_does_not_reach_a_row(L, S, window, sinks, dtype):
     import hbq_b200 as h
     q, k, v = _inputs(1, L, 4, 2, S, 64, dtype, 5)
@@ -145,7 +145,7 @@ def test_what_a_mask_hides_does_not_reach_a_row(L, S, window, sinks, dtype):
 
 
 @pytest.mark.parametrize("peak,scale", [(0.0, None), (30.0, None), (1.0, 3.0), (1.0, 1e-4), (200.0, 1.0)])
-@pytest.mark.parametrize("L", [1, 70])
+@pytest.mark.parametrize("L", [1, 70, 90])
 def test_flat_and_peaked_weights(peak, scale, L):
     import hbq_b200 as h
     for dtype in (torch.float16, torch.bfloat16):
@@ -154,7 +154,7 @@ def test_flat_and_peaked_weights(peak, scale, L):
         _close(got, *_reference(q, k, v, _all(600, 2), None, 300, 2, scale or 1 / math.sqrt(128)))
 
 
-@pytest.mark.parametrize("L", [1, 50])
+@pytest.mark.parametrize("L", [1, 50, 90])
 def test_layouts(L):
     import hbq_b200 as h
     q, k, v = _inputs(2, L, 8, 2, 90, 64, torch.float16, 3)
@@ -187,7 +187,8 @@ def test_layouts(L):
 
 
 PREFIX = [(2, 1, 4, 2, 100, 7, 64), (8, 1, 32, 8, 1000, 50, 128), (5, 1, 3, 3, 129, 1, 80), (64, 1, 8, 2, 700, 33, 128), (3, 17, 8, 2, 300, 40, 64), (2, 130, 4, 1, 257, 130, 128),
-          (1, 1, 1, 1, 1, 1, 8), (1, 300, 4, 4, 64, 300, 96), (33, 1, 20, 1, 4000, 5, 112), (70, 2, 6, 2, 900, 20, 72)]
+          (1, 1, 1, 1, 1, 1, 8), (1, 300, 4, 4, 64, 300, 96), (33, 1, 20, 1, 4000, 5, 112), (70, 2, 6, 2, 900, 20, 72), (64, 1, 8, 2, 3000, 33, 128),
+          (8, 1, 32, 8, 5000, 50, 128), (3, 17, 8, 2, 3000, 40, 64), (5, 1, 3, 3, 20000, 1, 80), (2, 90, 24, 3, 600, 95, 96)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
@@ -235,7 +236,7 @@ def test_of_nothing():
     z = lambda *s: torch.empty(s, device="cuda").half()  # noqa: E731
     assert h.window_attention(z(0, 3, 4, 64), z(0, 2, 5, 64), z(0, 2, 5, 64)).shape == (0, 3, 4, 64)
     assert h.window_attention(z(2, 0, 4, 64), z(2, 2, 5, 64), z(2, 2, 5, 64)).shape == (2, 0, 4, 64)
-    for L in (1, 60):
+    for L in (1, 60, 200):
         got = h.window_attention(torch.ones((2, L, 4, 64), device="cuda").half(), z(2, 2, 0, 64), z(2, 2, 0, 64))
         assert got.shape == (2, L, 4, 64) and not bool(got.any())
 
@@ -243,7 +244,7 @@ def test_of_nothing():
 @pytest.mark.parametrize("H,Hkv", [(64, 1), (96, 2), (40, 1)])
 def test_many_heads_of_one_key_head(H, Hkv):
     import hbq_b200 as h
-    for L, S in ((1, 700), (1, 40), (9, 300)):
+    for L, S in ((1, 700), (1, 40), (9, 300), (60, 300), (150, 150)):
         q, k, v = _inputs(2, L, H, Hkv, S, 64, torch.bfloat16, 8)
         lengths = _lengths([S, S - 7])
         got = h.window_attention(q, k, v, window=200, sinks=2, lengths=lengths)
@@ -268,7 +269,7 @@ def test_few_tokens_behind_a_prefix(B, L, H, Hkv):
 def test_outputs_of_any_alignment(step, H):
     """Rows of the output that are not 16 bytes apart, and outputs that begin off a 16-byte boundary."""
     import hbq_b200 as h
-    for L in (1, 40):
+    for L in (1, 40, 90):
         q, k, v = _inputs(2, L, H, 2, 90, 64, torch.float16, 3)
         want = h.window_attention(q, k, v)
         wide = torch.full((2, L, H, 64 + step), 9.0, device="cuda").half()
@@ -283,7 +284,7 @@ def test_windows_and_first_tokens_beyond_the_cache():
     """The same keys by another division of the work: each result is off by half a step (2^-12) of itself and of its weighted sum
     of |v|, which is below 3 here -- 2 * 2^-12 * 3 < 2^-9 between them."""
     import hbq_b200 as h
-    for L in (1, 50):
+    for L in (1, 50, 90):
         q, k, v = _inputs(2, L, 8, 2, 90, 64, torch.float16, 3)
         want = h.window_attention(q, k, v)
         for window, sinks in ((90, 0), (2 ** 40, 5), (2 ** 62, 2 ** 62), (1, 90), (1, 2 ** 62)):
@@ -334,12 +335,12 @@ def test_a_cache_beyond_32_bit_offsets():
     cache = torch.zeros((B, Hkv, S, D), device="cuda", dtype=torch.float16)
     g = torch.Generator(device="cuda").manual_seed(1)
     n = S - 3
-    for L in (1, 20):
+    for L in (1, 20, 120):
         q = torch.randn((B, L, 4, D), device="cuda", generator=g).half()
-        part = torch.randn((B, Hkv, 333, D), device="cuda", generator=g).half()
-        cache[:, :, n - 333:n] = part
+        part = torch.randn((B, Hkv, 433, D), device="cuda", generator=g).half()
+        cache[:, :, n - 433:n] = part
         got = h.window_attention(q, cache, cache, window=300, lengths=_all(n, B))
-        _close(got, *_reference(q, part, part, _all(333, B), None, 300, 0, 1 / math.sqrt(D)))
+        _close(got, *_reference(q, part, part, _all(433, B), None, 300, 0, 1 / math.sqrt(D)))
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
