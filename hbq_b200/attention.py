@@ -38,7 +38,7 @@ def _counts(name: str, t: Optional[torch.Tensor], B: int) -> Optional[torch.Tens
 def _run(what: str, q, k, v, prefix_k, prefix_v, window: int, sinks: int, scale: Optional[float], lengths, starts, out) -> torch.Tensor:
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1]) if q.dim() == 4 and q.shape[-1] else 1.0
-    if out is None and q.is_cuda and window >= 0 and sinks >= 0 and scale > 0:
+    if out is None and q.is_cuda and window >= 0 and sinks >= 0 and scale > 0 and math.isfinite(scale):
         y = _lib.host().attention(q, k, v, prefix_k, prefix_v, window, sinks, scale, lengths, starts)
         if isinstance(y, torch.Tensor):
             return y

@@ -12,6 +12,13 @@
 // are left out; the mask is applied only in tiles that hide some key from some row.  There the weights hold zeros, and a
 // zero times an infinity or a NaN of a hidden value would still reach the sum: such values are set to zero in shared memory
 // before the product, and the rows that do see them get them added at the end.
+//
+// What bounds it: per pair of 128 x 128 tiles the products take 2048 cycles at heads of 128, and shared memory delivers their operands in
+// as many; the powers of two take 2048 on the special-function unit, a quarter of which is computed on the FMA pipe instead.  A
+// row tile's softmax (some 1700 cycles) and the products it waits for (1024 and 300 of hand-over) follow one another, since the weights
+// lie on the scores: tensor memory has no room for both.  The tensor pipe is busy 55 % of the time.  8192 tokens, 32 / 8 heads of
+// 128, bf16: all keys 456 us, 1200 TFLOP/s; window of 4096 375 us, 1100 of visible pairs; under a sustained load, where the
+// power cap holds the clock near 1.65 GHz, 444 us.  A block of one key tile takes some 7 us.
 #include "attention_dev.cuh"
 #include "tc_dev.cuh"
 
@@ -36,8 +43,9 @@ struct TcTask {
     int prefix, k_by_head, k_by_seq, v_by_head, v_by_seq, vector_out, tma_out;
 };
 
-// Bounded wait of one thread, and of a warp by its lane 0 (a poll by all lanes is 32 accesses to the barrier's word, beside
-// the tensor core's own use of shared memory).
+// Bounded waits of one thread and of a warp.  One thread waits for, issues and commits the products (a warp whose lanes vote on each
+// wait: 944 -> 1024 TFLOP/s with 8192 tokens, all keys); the rows' warps poll with all lanes (lane 0 and a shuffle: 606
+// and 536 us).
 __device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code)
 {
     #pragma unroll 1
@@ -306,8 +314,8 @@ __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_const
                     tc_fence_after();
                     output(1, vs, j > 0);
                 }
-                tc_commit(kv_empty + 8 * vs);
-                if (more) {
+                if (more) {                                  // (behind the last values nothing is loaded)
+                    tc_commit(kv_empty + 8 * vs);
                     if (two) scores(1, ks);
                     tc_commit(kv_empty + 8 * ks);
                     next();

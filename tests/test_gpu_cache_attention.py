@@ -291,13 +291,13 @@ def test_windows_and_first_tokens_beyond_the_cache():
             _close(h.window_attention(q, k, v, window=window, sinks=sinks), want.double(), 2.0 ** -10 * want.double().abs() + 2.0 ** -9)
 
 
-@pytest.mark.parametrize("L", [1, 90])
-def test_streams_graphs_and_two_calls_at_once(L):
+@pytest.mark.parametrize("L,S,P", [(1, 5000, 3000), (90, 5000, 3000), (1, 900, 300), (3, 100, 50)])
+def test_streams_graphs_and_two_calls_at_once(L, S, P):
     import hbq_b200 as h
-    q, k, v = _inputs(2, L, 8, 2, 5000, 128, torch.bfloat16, 3)
-    pk, pv = (torch.randn((2, 3000, 128), device="cuda").bfloat16() for _ in range(2))
-    lengths = _lengths([5000, 1234])
-    call = lambda: (h.window_attention(q, k, v, window=4000, sinks=4, lengths=lengths), h.shared_prefix_attention(q, pk, pv, k, v, lengths=lengths))  # noqa: E731
+    q, k, v = _inputs(2, L, 8, 2, S, 128, torch.bfloat16, 3)
+    pk, pv = (torch.randn((2, P, 128), device="cuda").bfloat16() for _ in range(2))
+    lengths = _lengths([S, S // 4])
+    call = lambda: (h.window_attention(q, k, v, window=S * 4 // 5, sinks=4, lengths=lengths), h.shared_prefix_attention(q, pk, pv, k, v, lengths=lengths))  # noqa: E731
     want = call()
     assert all(torch.equal(a, b) for a, b in zip(call(), want))           # the same bits every time
     torch.cuda.synchronize()
@@ -312,7 +312,7 @@ def test_streams_graphs_and_two_calls_at_once(L):
     for g in graphs:
         with torch.cuda.graph(g):
             outs.append(call())
-    k.copy_(torch.randn_like(k)); lengths.copy_(_lengths([4321, 5000]))
+    k.copy_(torch.randn_like(k)); lengths.copy_(_lengths([S * 6 // 7, S]))
     want = call()
     torch.cuda.synchronize()
     for s, g in zip(streams, graphs):                                      # two graphs in flight at once
