@@ -231,6 +231,50 @@ def test_shared_prefix_edges():
     assert not bool(got[1, 20:].any()) and not bool(got[2].any())
 
 
+@pytest.mark.parametrize("B,L,H,Hkv", [(8, 40, 8, 2), (200, 1, 8, 2), (1, 200, 6, 2), (3, 70, 6, 6), (300, 2, 3, 1)])
+@pytest.mark.parametrize("P", [100, 1000])
+def test_a_prefix_alone(B, L, H, Hkv, P):
+    """No keys of the sequences' own: the prefix' kernel writes the output, in any layout."""
+    import hbq_b200 as h
+    q, none, _ = _inputs(B, L, H, Hkv, 0, 64, torch.float16, P)
+    pk, pv = (torch.randn((Hkv, P, 64), device="cuda").half() for _ in range(2))
+    lengths, starts = _all(0, B), _lengths([-L if b % 3 else -L // 2 - 1 for b in range(B)])      # rows from position 0 on are padding
+    for st in (None, starts):
+        o, tol = _reference(q, none, none, lengths, st, 0, 0, 1 / 8, (pk, pv))
+        _close(h.shared_prefix_attention(q, pk, pv, none, none, starts=st), o, tol)
+        wide = torch.full((B, L + 1, H + 1, 72), 3.0, device="cuda").half()
+        h.shared_prefix_attention(q, pk, pv, none, none, starts=st, out=wide[:, 1:, :-1, :64])
+        _close(wide[:, 1:, :-1, :64], o, tol)
+        assert bool((wide[:, 0] == 3).all()) and bool((wide[:, :, -1] == 3).all()) and bool((wide[..., 64:] == 3).all())
+        byhead = torch.empty((H, L, B, 64), device="cuda").half()
+        h.shared_prefix_attention(q, pk, pv, none, none, starts=st, out=byhead.permute(2, 1, 0, 3))
+        _close(byhead.permute(2, 1, 0, 3), o, tol)
+
+
+def test_queries_beyond_32_bit_offsets():
+    """A prompt whose queries, keys turned in place and outputs pass 2^31 elements, against single rows of it."""
+    import hbq_b200 as h
+    L, H, Hkv, D = 540001, 32, 8, 128
+    if torch.cuda.get_device_properties(0).total_memory < 60e9:
+        pytest.skip("needs 20 GB")
+    g = torch.Generator(device="cuda").manual_seed(2)
+    q = torch.empty((1, L, H, D), device="cuda", dtype=torch.float16)
+    for part in q.split(60000, 1):
+        part.copy_(torch.randn(part.shape, device="cuda", generator=g, dtype=torch.float16))
+    k, v = (torch.randn((1, Hkv, L, D), device="cuda", generator=g, dtype=torch.float16) for _ in range(2))
+    got = h.window_attention(q, k, v, window=200, sinks=3)
+    f, _ = h.rope_frequencies(D, 500000.0, device="cuda")
+    pos = torch.arange(L, device="cuda")
+    some = [0, 1, 1023, 199999, 524287, 524288, 530000, L - 1]
+    for p in some:
+        keys = list(range(min(3, max(0, p - 199)))) + list(range(max(0, p - 199), p + 1))
+        o, tol = _reference(q[:, p:p + 1], k[:, :, keys], v[:, :, keys], _all(len(keys), 1), None, 0, 0, 1 / math.sqrt(D))
+        _close(got[:, p:p + 1], o, tol)
+    rows = q[:, some].clone()
+    h.rope_rotate(q, f, pos, out=q)
+    assert torch.equal(q[:, some], h.rope_rotate(rows, f, pos[some]))
+
+
 def test_of_nothing():
     import hbq_b200 as h
     z = lambda *s: torch.empty(s, device="cuda").half()  # noqa: E731
