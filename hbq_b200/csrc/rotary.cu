@@ -109,7 +109,7 @@ __device__ __forceinline__ void unpack(uint4 r0, uint4 r1, bool apart, float2 (&
 //
 // Bytes in flight are what it needs: a warp's next heads are loaded before it works on the present ones, and its first ones
 // before the block's angles are known (16384 tokens of 32 heads of 128: 47 us, 5.7 TB/s; 32 + 8 heads with
-// the norm: 67 us, 5.0 TB/s).
+// the norm: 66 us, 5.1 TB/s).
 template <class E, int LANES, bool NORM>
 __global__ void __launch_bounds__(WARPS * 32, 6) rotary_kernel(const __grid_constant__ RotaryArgs a)
 {
@@ -145,7 +145,8 @@ __global__ void __launch_bounds__(WARPS * 32, 6) rotary_kernel(const __grid_cons
         return v;
     };
     const double* freq = behind_wait(a.inv_freq);
-    float2 cs[4], neg[4];                          // cosines and negated sines of the lane's pairs, two and two
+    // the lane's pairs, two and two: (u, v) -> (u uu + v vu, v vv + u uv), cosines and sines times the weights where there is a norm
+    float2 uu[4], vu[4], vv[4], uv[4];
     bool ready = false;
     #pragma unroll 1
     for (int j = 0; j < 2; ++j) {
@@ -154,14 +155,10 @@ __global__ void __launch_bounds__(WARPS * 32, 6) rotary_kernel(const __grid_cons
         const E* from = static_cast<const E*>(x.data) + (int64_t)b * x.sb + (int64_t)t * x.st;
         E* to = static_cast<E*>(x.out) + (int64_t)b * x.ob + (int64_t)t * x.ot;
         Item next = load(x, from, to, any ? heads : 0, g);
-        float2 wu[4], ww[4];                       // the weights, as the values below
-        if (NORM) {
-            uint4 u0 = make_uint4(0, 0, 0, 0), u1 = u0;
-            if (in_head && g < groups) {
-                u0 = *reinterpret_cast<const uint4*>(static_cast<const E*>(x.weight) + d0);
-                u1 = *reinterpret_cast<const uint4*>(static_cast<const E*>(x.weight) + d1);
-            }
-            unpack<E>(u0, u1, apart, wu, ww);
+        uint4 w0 = make_uint4(0, 0, 0, 0), w1 = w0;
+        if (NORM && in_head && g < groups) {
+            w0 = *reinterpret_cast<const uint4*>(static_cast<const E*>(x.weight) + d0);
+            w1 = *reinterpret_cast<const uint4*>(static_cast<const E*>(x.weight) + d1);
         }
         if (!ready) {                              // (the first loads are on their way)
             ready = true;
@@ -171,13 +168,26 @@ __global__ void __launch_bounds__(WARPS * 32, 6) rotary_kernel(const __grid_cons
                 for (uint32_t i = lane; i < half; i += 32) angles[i] = turn(position, freq[i], a.factor);
             }
             __syncwarp();
-            if (turns && any) {
+            if (!NORM && turns && any) {
                 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float2 p = angles[8 * c + 2 * i], q = angles[8 * c + 2 * i + 1];
-                    cs[i] = make_float2(p.x, q.x);
-                    neg[i] = make_float2(-p.y, -q.y);
+                    uu[i] = make_float2(p.x, q.x);
+                    vu[i] = make_float2(-p.y, -q.y);
                 }
+            }
+        }
+        if (NORM) {
+            float2 wu[4], wv[4];
+            unpack<E>(w0, w1, apart, wu, wv);
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float2 p = make_float2(1.f, 0.f), q = p;
+                if (turns && any) { p = block_angles[warp][8 * c + 2 * i]; q = block_angles[warp][8 * c + 2 * i + 1]; }
+                uu[i] = mul2(make_float2(p.x, q.x), wu[i]);
+                uv[i] = mul2(make_float2(p.y, q.y), wu[i]);
+                vv[i] = mul2(make_float2(p.x, q.x), wv[i]);
+                vu[i] = mul2(make_float2(-p.y, -q.y), wv[i]);
             }
         }
         for (; g < groups && any; g += step) {
@@ -185,6 +195,7 @@ __global__ void __launch_bounds__(WARPS * 32, 6) rotary_kernel(const __grid_cons
             next = load(x, from, to, heads, g + step);
             float2 u[4], v[4];
             unpack<E>(cur.u0, cur.u1, apart, u, v);
+            float2 ss = make_float2(1.f, 1.f);
             if (NORM) {
                 float2 q = make_float2(0.f, 0.f);
                 #pragma unroll
@@ -193,17 +204,22 @@ __global__ void __launch_bounds__(WARPS * 32, 6) rotary_kernel(const __grid_cons
                 #pragma unroll
                 for (int m = LANES / 2; m; m >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, m);
                 s = rsqrtf(fmaf(s, a.inv_D, a.eps));
-                const float2 ss = make_float2(s, s);
-                #pragma unroll
-                for (int i = 0; i < 4; ++i) { u[i] = mul2(u[i], mul2(ss, wu[i])); v[i] = mul2(v[i], mul2(ss, ww[i])); }
+                ss = make_float2(s, s);
             }
             if (turns) {
                 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float2 r = fma2(u[i], cs[i], mul2(v[i], neg[i]));
-                    v[i] = fma2(v[i], cs[i], mul2(u[i], make_float2(-neg[i].x, -neg[i].y)));
+                    const float2 r = fma2(u[i], uu[i], mul2(v[i], vu[i]));
+                    v[i] = fma2(v[i], NORM ? vv[i] : uu[i], mul2(u[i], NORM ? uv[i] : make_float2(-vu[i].x, -vu[i].y)));
                     u[i] = r;
                 }
+            } else if (NORM) {
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) { u[i] = mul2(u[i], uu[i]); v[i] = mul2(v[i], vv[i]); }
+            }
+            if (NORM) {
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) { u[i] = mul2(u[i], ss); v[i] = mul2(v[i], ss); }
             }
             if (cur.out) {
                 if (apart) {
