@@ -103,7 +103,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     the keys up to p that are among the last ``window`` ones, itself included, or among the first ``sinks`` of the sequence;
     ``window=0``: all of them.  A row that sees nothing (p below 0), and a row behind its sequence's end (p >= ``lengths[b]``, the
     padding of a batch of prompts), is 0.  What the cache holds behind a sequence's end, or where a row's mask hides it, does
-    not matter, infinities and NaNs among it.  ``L = 1`` is a decode step.  ``scale`` defaults to ``1 / sqrt(D)``."""
+    not matter, infinities and NaNs among it.  ``L = 1`` is a decode step.  ``scale`` defaults to ``1 / sqrt(D)``.  The result may be given as
+    ``out``, of any strides with a dense last axis, which overlaps no input."""
     return _run("window_attention", q, k, v, None, None, int(window), int(sinks), scale, lengths, starts, out)
 
 
