@@ -312,7 +312,8 @@ __global__ void __launch_bounds__(RW * 32, BLOCKS_PER_SM) attention_rows_kernel(
             for (int e = 0; e < 2; ++e) {
                 const float w0 = exp2_fast(fmaf(s[e][2 * r], c, off)), w1 = exp2_fast(fmaf(s[e][2 * r + 1], c, off));
                 l[r] += w0 + w1;
-                // the weights as two numbers of the values' type, so that their rounding does not reach the result
+                // the weights as two numbers of the values' type, so that their rounding does not reach the result (the second may
+                // be negative, and makes a NaN of an infinity among the values: specials_of)
                 hi[2 * e + r] = Mma<E>::pack(w0, w1);
                 const float2 back = Mma<E>::unpack(hi[2 * e + r]);
                 rest[2 * e + r] = Mma<E>::pack(w0 - back.x, w1 - back.y);
@@ -348,7 +349,9 @@ __global__ void __launch_bounds__(RW * 32, BLOCKS_PER_SM) attention_rows_kernel(
             part_sum(a, at, a.part0)[d] = sum;
             if (d == 0) *part_weight(a, at, a.part0) = make_float2(top, weight);
         } else {
-            Mma<E>::store(a.out, (int64_t)b * a.os[0] + (int64_t)i * a.os[1] + (int64_t)(h0 + row) * a.os[2] + d, weight == 0.f ? 0.f : sum / weight);
+            float y = weight == 0.f ? 0.f : sum / weight;
+            if (y != y && weight == weight) y = specials_of<E, 1>(a, b, i, hk, d & ~7u, 0, 1, 1u << (d & 7)).in_place_of(y, d & 7);
+            Mma<E>::store(a.out, (int64_t)b * a.os[0] + (int64_t)i * a.os[1] + (int64_t)(h0 + row) * a.os[2] + d, y);
         }
     };
     float* block = reinterpret_cast<float*>(smem + Sh::JOIN);
@@ -436,7 +439,7 @@ __global__ void __launch_bounds__(RW * 32, BLOCKS_PER_SM) attention_rows_kernel(
 // sums relative to the largest.  A chain of dependent loads, bound by their latency: the blocks of a group come from its
 // table entry, and with few rows four warps share a row's parts (8 rows of 37 parts: 8.4 -> 5 us).
 template <class E, int W>
-__global__ void __launch_bounds__(128) attention_join_kernel(const __grid_constant__ AttnArgs a, uint32_t tiles)
+__global__ void __launch_bounds__(128, W > 1 ? 16 : 12) attention_join_kernel(const __grid_constant__ AttnArgs a, uint32_t tiles)
 {
     __shared__ float sums[W > 1 ? W : 1][128], weights[W > 1 ? W : 1];
     grid_dependency_wait();
@@ -472,7 +475,8 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
         float f = 0.f;
         if (s0 + lane * W < count) {
             const float2 ml = weight_of(s0 + lane * W);
-            if (ml.y != 0.f) { f = exp2_fast(ml.x - ref); weight = fmaf(ml.y, f, weight); }
+            // (no part that saw a key counts for nothing: its sum may be an infinity.  The smallest number there is adds below 2^-24 to others)
+            if (ml.y != 0.f) { f = fmaxf(exp2_fast(ml.x - ref), __uint_as_float(1u)); weight = fmaf(ml.y, f, weight); }
         }
         const int end = min(32, (count - s0 + W - 1) / W);
         #pragma unroll 8
@@ -500,10 +504,25 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
         }
     }
     const uint32_t b = token / a.L, i = token - b * a.L;
+    const int64_t at = (int64_t)b * a.os[0] + (int64_t)i * a.os[1] + (int64_t)h * a.os[2];
+    bool odd = false;
     if (in) {
         #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            Mma<E>::store(a.out, (int64_t)b * a.os[0] + (int64_t)i * a.os[1] + (int64_t)h * a.os[2] + lane * 4 + e, weight == 0.f ? 0.f : sum[e] / weight);
+        for (int e = 0; e < 4; ++e) {
+            const float y = weight == 0.f ? 0.f : sum[e] / weight;
+            odd |= y != y;
+            Mma<E>::store(a.out, at + lane * 4 + e, y);
+        }
+    }
+    uint32_t lanes = __ballot_sync(0xFFFFFFFFu, odd && weight == weight);
+    while (lanes) {                                                  // eight columns with a NaN among them: two lanes'
+        const int piece = (__ffs(lanes) - 1) / 2;
+        lanes &= ~(3u << (2 * piece));
+        Specials s = specials_of<E, 1>(a, b, i, h / a.G, piece * 8, lane, 32, 0xFFu);
+        s.above = __reduce_or_sync(0xFFFFFFFFu, s.above);
+        s.below = __reduce_or_sync(0xFFFFFFFFu, s.below);
+        __syncwarp();                                                // (behind the stores of the same values above)
+        if (lane < 8 && ((s.above | s.below) >> lane & 1u)) Mma<E>::store(a.out, at + piece * 8 + lane, s.in_place_of(0.f, lane));
     }
 }
 
