@@ -523,7 +523,7 @@ __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_const
                                 #pragma unroll 1
                                 for (int e = 0; e < 32; ++e) {
                                     if (32 * k + e >= (int)a.D) break;
-                                    const float x = Word<E>::up(reinterpret_cast<const uint16_t*>(v)[j * vstep + 32 * k + e]);
+                                    const float x = Word<E>::up(__ldcg(reinterpret_cast<const uint16_t*>(v) + j * vstep + 32 * k + e));     // (begin_beside)
                                     if (!isfinite(x)) {
                                         #pragma unroll
                                         for (int z = 0; z < 32; ++z) if (z == e) o[z] += x;
