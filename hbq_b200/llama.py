@@ -157,22 +157,33 @@ class QLlamaAttention(nn.Module):
             return qk_norm_rope(q, k, self.q_norm, self.k_norm, self.eps, freq, pos, self.interleaved, factor)
         return tuple(rope_rotate(t, freq, pos, self.interleaved, factor) for t in (q, k))
 
+    def _in_runs(self, q_len: int) -> bool:
+        """A causal prefill is cut into runs of ``query_chunk`` queries."""
+        c = self.query_chunk
+        return q_len > c and q_len % c == 0 and c % 128 == 0
+
     def _windowed(self, Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor) -> torch.Tensor:
         """Causal attention, of a window and the first tokens where there is one, on ``[B, H, T, D]``, as o_proj's rows.  Where the probabilities are
-        quantised, or heads are longer than the one-pass kernel's, it is ``softmax_quantize``'s with the mask in memory."""
+        quantised, or heads are longer than the one-pass kernel's, it is ``softmax_quantize``'s with the mask in memory, a run of
+        queries at a time against the keys up to its end, as the plain causal prefill's."""
         B, H, T, D = Q.shape
         aq = self.attn_wgt_quantizer if self.quant_attn_wgt else None
         if aq is None and D % 8 == 0 and D <= 128:
             return window_attention(Q.transpose(1, 2), K, V, window=self.window, sinks=self.sinks).view(B * T, H * D)
-        j = torch.arange(T, device=Q.device)
-        hidden = j[None] > j[:, None]
-        if self.window > 0:
-            hidden = hidden | ((j[None] <= j[:, None] - self.window) & (j[None] >= self.sinks))
-        mask = torch.zeros((1, 1, T, T), dtype=Q.dtype, device=Q.device).masked_fill_(hidden, float("-inf"))
-        scores = torch.matmul(Q.reshape(B, K.shape[1], -1, D), K.transpose(-1, -2))
-        P = softmax_quantize(scores.view(B, H, T, T), 1.0 / math.sqrt(D), aq, mask=mask)
-        O = torch.matmul(P.view(scores.shape), V).view(B, H, T, D)
-        return O.transpose(1, 2).reshape(B * T, H * D)
+        Hkv, c = K.shape[1], self.query_chunk if self._in_runs(T) else T
+        Q5 = Q.reshape(B, Hkv, H // Hkv, T, D)
+        O4 = torch.empty((B, T, H, D), dtype=Q.dtype, device=Q.device)
+        for t0 in range(0, T, c):
+            t1 = t0 + c
+            i, j = torch.arange(t0, t1, device=Q.device)[:, None], torch.arange(t1, device=Q.device)[None]
+            hidden = j > i
+            if self.window > 0:
+                hidden = hidden | ((j <= i - self.window) & (j >= self.sinks))
+            mask = torch.zeros((1, 1, c, t1), dtype=Q.dtype, device=Q.device).masked_fill_(hidden, float("-inf"))
+            scores = torch.matmul(Q5[:, :, :, t0:t1].reshape(B, Hkv, -1, D), K[:, :, :t1].transpose(-1, -2))
+            P = softmax_quantize(scores.view(B, H, c, t1), 1.0 / math.sqrt(D), aq, mask=mask)
+            O4[:, t0:t1] = torch.matmul(P.view(scores.shape), V[:, :, :t1]).view(B, H, c, D).transpose(1, 2)
+        return O4.view(B * T, H * D)
 
     def forward(self, x: torch.Tensor, bsz: int, q_len: int, cos: torch.Tensor, sin: torch.Tensor,
                 input_quantized: bool = False) -> torch.Tensor:
@@ -188,9 +199,9 @@ class QLlamaAttention(nn.Module):
             q, k = (t.view(bsz, q_len, -1) for t in self._turned(q.view(bsz, q_len, H, D), k.view(bsz, q_len, Hkv, D), q_len))
             cos = sin = None
         c = self.query_chunk
-        in_runs = q_len > c and q_len % c == 0 and c % 128 == 0 and cos is not None and self.window == 0
+        in_runs = self._in_runs(q_len) and self.window == 0
         Q = Qr = None
-        if in_runs and self.quant_post_rope_q and calls_only_its_format(self.q_proj.aq):
+        if in_runs and cos is not None and self.quant_post_rope_q and calls_only_its_format(self.q_proj.aq):
             Qr = kvcache.quantize_q_runs(q, H, G, c, self.q_proj.aq, cos, sin)
         if Qr is not None:
             pass
