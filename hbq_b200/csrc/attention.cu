@@ -13,7 +13,8 @@ int check(const hbq_attention* p)
     if (p->H % p->Hkv || !(p->scale > 0.f) || !isfinite(p->scale)) return HBQ_ERR_ARG;
     if (p->B == 0 || p->L == 0 || p->H == 0) return HBQ_OK;
     if (!p->q || !p->out || (p->S > 0 && (!p->k || !p->v)) || (p->P > 0 && (!p->prefix_k || !p->prefix_v))) return HBQ_ERR_ARG;
-    if (p->D > 128 || (p->D % 8) || p->S > 0x7FFFFFFFll || p->P > 0x7FFFFFFFll || p->L > 0x7FFFFFFFll || p->B > 65535 || p->H > 65535 ||
+    // (key positions are ints in the kernels, and a tile may end up to 127 behind the last key)
+    if (p->D > 128 || (p->D % 8) || p->S > 0x7FFFFF00ll || p->P > 0x7FFFFF00ll || p->L > 0x7FFFFFFFll || p->B > 65535 || p->H > 65535 ||
         p->B * p->H > (1ll << 40) / p->L)
         return HBQ_ERR_UNSUPPORTED;
     int64_t s = 0;

@@ -1,0 +1,27 @@
+"""CPU: what the C entry of the attention refuses before any launch, at the ends of its ranges."""
+import ctypes
+
+import pytest
+
+pytest.importorskip("torch")
+ARG, UNSUPPORTED, ALIGN = -1, -2, -4
+I3, I2 = ctypes.c_int64 * 3, ctypes.c_int64 * 2
+
+
+def _run(**kw):
+    """Two sequences of four tokens; the pointers are never followed."""
+    from hbq_b200 import _lib
+    p = ctypes.c_void_p(1 << 20)
+    a = _lib.Attention(p, p, p, p, 2, 4, 4, 2, 9, 64, I3(1024, 256, 64), I3(64 * 18, 64 * 9, 64), I3(64 * 18, 64 * 9, 64), I3(1024, 256, 64),
+                       None, None, None, None, 0, I2(0, 0), I2(0, 0), 0, 0, 0.125, 0)
+    for n, v in kw.items():
+        setattr(a, n, v)
+    return _lib.lib().hbq_attention_run(ctypes.byref(a), None, 0, None)
+
+
+def test_key_counts_next_to_32_bits():
+    """Key positions are 32-bit numbers in the kernels, and a tile of 128 keys may end behind the last key."""
+    p = ctypes.c_void_p(1 << 20)
+    for n in (2 ** 31 - 1, 2 ** 31 - 128, 2 ** 31 - 255):
+        assert _run(S=n) == UNSUPPORTED
+        assert _run(P=n, prefix_k=p, prefix_v=p, pk_stride=I2(64, 64), pv_stride=I2(64, 64)) == UNSUPPORTED
