@@ -24,7 +24,15 @@ int check(const hbq_attention* p)
     if (p->S > 0) u |= reinterpret_cast<uintptr_t>(p->k) | reinterpret_cast<uintptr_t>(p->v);
     if (p->P > 0) u |= reinterpret_cast<uintptr_t>(p->prefix_k) | reinterpret_cast<uintptr_t>(p->prefix_v);
     const bool same_keys = (p->S > 1 && (p->k_stride[2] <= 0 || p->v_stride[2] <= 0)) || (p->P > 1 && (p->pk_stride[1] <= 0 || p->pv_stride[1] <= 0));
-    return (s % 8) || (u & 15) || same_keys ? HBQ_ERR_ALIGN : HBQ_OK;
+    // (the copies' maps take an axis without a positive stride for one element repeated, of a cache, or a dense one, of the output)
+    bool down = false;
+    for (int i = 0; i < 2; ++i) {
+        down |= p->S > 0 && (i ? p->Hkv : p->B) > 1 && (p->k_stride[i] < 0 || p->v_stride[i] < 0);
+        down |= p->P > 0 && (i ? p->P : p->Hkv) > 1 && (p->pk_stride[i] < 0 || p->pv_stride[i] < 0);
+    }
+    const int64_t outs[3] = {p->B, p->L, p->H};
+    for (int i = 0; i < 3; ++i) down |= outs[i] > 1 && p->out_stride[i] <= 0;
+    return (s % 8) || (u & 15) || same_keys || down ? HBQ_ERR_ALIGN : HBQ_OK;
 }
 
 bool nothing(const hbq_attention* p) { return p->B == 0 || p->L == 0 || p->H == 0; }

@@ -368,7 +368,8 @@ int hbq_qk_norm_rope(const hbq_heads* q, const hbq_heads* k, const hbq_rotary* r
  *   A row that sees nothing becomes 0, and so does a row at or behind its sequence's end (p >= lengths[b]).  Keys and
  *   values that a row does not see, whatever they hold, do not reach it.
  * prefix: keys and values [Hkv, P, D] in front of every sequence, seen by every row that is not behind its sequence's end.
- * D a multiple of 8 up to 128, S and P at most 2^31 - 256; pointers 16-byte aligned, strides of q, k, v multiples of 8.
+ * D a multiple of 8 up to 128, S and P at most 2^31 - 256; pointers 16-byte aligned, strides of q, k, v multiples of 8,
+ * none of k, v negative (0, but for the keys: an axis of the same elements), those of out positive.
  * workspace: hbq_attention_workspace_bytes(...) bytes (0: none), 32-byte aligned, contents irrelevant. */
 typedef struct hbq_attention {
     const void *q, *k, *v;

@@ -25,3 +25,22 @@ def test_key_counts_next_to_32_bits():
     for n in (2 ** 31 - 1, 2 ** 31 - 128, 2 ** 31 - 255):
         assert _run(S=n) == UNSUPPORTED
         assert _run(P=n, prefix_k=p, prefix_v=p, pk_stride=I2(64, 64), pv_stride=I2(64, 64)) == UNSUPPORTED
+
+
+def test_strides_that_the_kernels_maps_cannot_hold():
+    """Caches with negative strides, outputs whose elements are not separate: the copies' maps would take the axis for a dense one."""
+    p = ctypes.c_void_p(1 << 20)
+    for axis in range(3):
+        down = [64 * 18, 64 * 9, 64]
+        down[axis] *= -1
+        assert _run(k_stride=I3(*down)) == ALIGN and _run(v_stride=I3(*down)) == ALIGN
+        for s in (0, -64):
+            out = [1024, 256, 64]
+            out[axis] = s
+            assert _run(out_stride=I3(*out)) == ALIGN
+    for axis in range(2):
+        down = [64 * 9, 64]
+        down[axis] *= -1
+        prefix = dict(P=9, prefix_k=p, prefix_v=p)
+        assert _run(**prefix, pk_stride=I2(*down), pv_stride=I2(64 * 9, 64)) == ALIGN
+        assert _run(**prefix, pk_stride=I2(64 * 9, 64), pv_stride=I2(*down)) == ALIGN
