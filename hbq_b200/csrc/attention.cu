@@ -10,7 +10,7 @@ int check(const hbq_attention* p)
 {
     if (!p || p->B < 0 || p->L < 0 || p->H < 0 || p->S < 0 || p->P < 0 || p->D <= 0 || p->Hkv <= 0 || p->sinks < 0) return HBQ_ERR_ARG;
     if (p->dtype != HBQ_DTYPE_F16 && p->dtype != HBQ_DTYPE_BF16) return HBQ_ERR_ARG;
-    if (p->H % p->Hkv || !(p->scale > 0.f) || !isfinite(p->scale)) return HBQ_ERR_ARG;
+    if (p->H % p->Hkv || !(p->scale > 0.f) || !isfinite(p->scale * 1.4426950408889634f)) return HBQ_ERR_ARG;
     if (p->B == 0 || p->L == 0 || p->H == 0) return HBQ_OK;
     if (!p->q || !p->out || (p->S > 0 && (!p->k || !p->v)) || (p->P > 0 && (!p->prefix_k || !p->prefix_v))) return HBQ_ERR_ARG;
     // (key positions are ints in the kernels, and a tile may end up to 127 behind the last key)

@@ -44,3 +44,9 @@ def test_strides_that_the_kernels_maps_cannot_hold():
         prefix = dict(P=9, prefix_k=p, prefix_v=p)
         assert _run(**prefix, pk_stride=I2(*down), pv_stride=I2(64 * 9, 64)) == ALIGN
         assert _run(**prefix, pk_stride=I2(64 * 9, 64), pv_stride=I2(*down)) == ALIGN
+
+
+def test_scales_at_the_ends_of_32_bits():
+    """The kernels work in powers of two: the scale times log2(e) has to be a number of 32 bits."""
+    for scale in (2.5e38, 3.4e38, 1e39, 0.0, 1e-46):
+        assert _run(scale=scale) == ARG
