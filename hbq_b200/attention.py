@@ -105,7 +105,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     padding of a batch of prompts), is 0.  What the cache holds behind a sequence's end, or where a row's mask hides it, does
     not matter, infinities and NaNs among it.  ``L = 1`` is a decode step.  ``scale`` defaults to ``1 / sqrt(D)``.  The result may be given as
     ``out``, of any strides with a dense last axis, which overlaps no input."""
-    return _run("window_attention", q, k, v, None, None, int(window), int(sinks), scale, lengths, starts, out)
+    # (a count beyond any cache, held to 64 bits)
+    return _run("window_attention", q, k, v, None, None, min(int(window), 2 ** 62), min(int(sinks), 2 ** 62), scale, lengths, starts, out)
 
 
 def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, k: torch.Tensor, v: torch.Tensor,

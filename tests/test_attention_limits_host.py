@@ -50,3 +50,29 @@ def test_scales_at_the_ends_of_32_bits():
     """The kernels work in powers of two: the scale times log2(e) has to be a number of 32 bits."""
     for scale in (2.5e38, 3.4e38, 1e39, 0.0, 1e-46):
         assert _run(scale=scale) == ARG
+
+
+@pytest.mark.parametrize("window,sinks", [(2 ** 64 + 5, 0), (5, 2 ** 64 + 3), (2 ** 70, 2 ** 70)])
+def test_windows_beyond_64_bits_are_all_of_the_cache(window, sinks, monkeypatch):
+    """A count beyond any cache means the whole of it and must not wrap around."""
+    import torch
+
+    from hbq_b200 import _lib, attention
+    seen = []
+
+    class Library:
+        @staticmethod
+        def hbq_attention_workspace_bytes(a):
+            seen.append((a._obj.window, a._obj.sinks))
+            return 0
+
+        @staticmethod
+        def hbq_attention_run(a, *rest):
+            return 0
+    monkeypatch.setattr(attention._lib, "lib", lambda: Library)
+    monkeypatch.setattr(attention, "_check_devices", lambda *a: None)
+    monkeypatch.setattr(attention, "_stream_ptr", lambda d: 0)
+    monkeypatch.setattr(_lib, "device_guard", lambda d: __import__("contextlib").nullcontext())
+    q, k = torch.zeros((1, 2, 2, 64), dtype=torch.float16), torch.zeros((1, 2, 9, 64), dtype=torch.float16)
+    attention.window_attention(q, k, k.clone(), window=window, sinks=sinks, out=torch.empty_like(q))
+    assert all(a == b if b < 9 else 9 <= a for a, b in zip(seen[0], (window, sinks)))
