@@ -33,6 +33,14 @@ __device__ __forceinline__ void sequence_of(const AttnArgs& a, uint32_t b, int64
     *first = a.starts ? (int64_t)__ldcg(a.starts + b) : len - (int64_t)a.L;
 }
 
+// Weights are 2^(score - maximum + SHIFT), and up to 2^GROWTH more until the sums are rescaled.  In fp16 2^4 keeps 16 times smaller
+// ones normal, and 2^(4 + 8) stays below the largest.  bf16 has room below, not above: its values go up to 2^128, and 2^24 of them
+// at weights of 2^-24 sum up inside 32 bits.
+constexpr float GROWTH = 8.f;
+template <class E> struct Weights;
+template <> struct Weights<__half> { static constexpr float SHIFT = 4.f; };
+template <> struct Weights<__nv_bfloat16> { static constexpr float SHIFT = -24.f; };
+
 __device__ __forceinline__ float exp2_fast(float x)
 {
     float y;

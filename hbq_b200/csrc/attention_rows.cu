@@ -31,7 +31,6 @@ namespace {
 // 131072, 64 of 1024); three of two stages 96, 122 and 59; one of four 102, 106 and 66.
 constexpr int RW = 4, STAGES = 3, GROUP = 16, BLOCKS_PER_SM = 2;
 constexpr uint32_t POLLS = 1u << 20;
-constexpr float SHIFT = 4.f, GROWTH = 8.f;          // as in the tensor-core kernel
 
 template <class E> struct Mma;
 template <> struct Mma<__half> {
@@ -155,6 +154,7 @@ template <class E, int NK>
 __global__ void __launch_bounds__(RW * 32, BLOCKS_PER_SM) attention_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ RowsMaps maps, uint32_t tiles)
 {
     using Sh = RowsShape<NK>;
+    constexpr float SHIFT = Weights<E>::SHIFT;
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ int64_t table[RW * 64 + 1];
     __shared__ __align__(8) uint64_t full[RW * STAGES];
@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(128, W > 1 ? 16 : 12) attention_join_kernel(co
         float f = 0.f;
         if (s0 + lane * W < count) {
             const float2 ml = weight_of(s0 + lane * W);
-            // (no part that saw a key counts for nothing: its sum may be an infinity.  The smallest number there is adds below 2^-24 to others)
+            // (no part that saw a key counts for nothing: its sum may be an infinity.  The smallest number there is, 2^-149, adds below 2^-20)
             if (ml.y != 0.f) { f = fmaxf(exp2_fast(ml.x - ref), __uint_as_float(1u)); weight = fmaf(ml.y, f, weight); }
         }
         const int end = min(32, (count - s0 + W - 1) / W);

@@ -6,7 +6,7 @@
 // the running maximum and sum of a softmax and writes the weights back over S in the values' type;  O += P V with P from tensor
 // memory.  While one warpgroup works on its tile's scores the tensor core multiplies for the other.
 // O stays in tensor memory; its rows are rescaled only when a row's maximum has grown by more than 2^8 in the weights
-// since the last time (weights up to 2^12 are as exact as weights up to 1, and the sum divides the factor out again).
+// since the last time (larger weights are as exact as weights up to 1, and the sum divides the factor out again).
 //
 // Keys come by TMA in a ring that keys and values share, from a cache of any strides.  Tiles that the masks of all rows hide
 // are left out; the mask is applied only in tiles that hide some key from some row.  There the weights hold zeros, and a
@@ -29,8 +29,6 @@ namespace {
 
 constexpr int TILE = 128, TCT = 320;
 constexpr uint32_t POLLS = 1u << 20;
-constexpr float SHIFT = 4.f;           // weights are 2^(x - maximum + 4): in fp16 that keeps 16 times smaller ones normal
-constexpr float GROWTH = 8.f;          // in powers of two; 2^(4 + 8) stays below fp16's largest
 
 template <int DP> struct TcShape {
     static constexpr int HALVES = DP / 64;
@@ -189,6 +187,7 @@ __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_const
                                                               const __grid_constant__ AttnArgs a, const __grid_constant__ TcTask task)
 {
     using Sh = TcShape<DP>;
+    constexpr float SHIFT = Weights<E>::SHIFT;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     const uint32_t qs = base, ring = base + Sh::Q, ctrl = ring + Sh::NS * Sh::STAGE;

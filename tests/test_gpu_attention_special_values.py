@@ -105,3 +105,27 @@ def test_values_written_just_before(L, P):
         want = plain.clone()
         want[:, odd, :, n] = INF if n % 2 else -INF
         assert torch.equal(o, want)
+
+
+@pytest.mark.parametrize("size", [3e38, 1e-33])
+@pytest.mark.parametrize("B,L,H,Hkv,S,P,window,sinks", CASES)
+def test_values_at_the_ends_of_bf16(B, L, H, Hkv, S, P, window, sinks, size):
+    """Values up to bf16's largest, and values near its smallest: a mean of them stays in range, and so has the sum it is made of.
+    Tolerance: half a step (2^-8) of the result for its rounding, the same of sum w |v| for the weights' rounding, and 2^-12 of that
+    for the scores' 32-bit sums and the additions; half of bf16's smallest normal number where the results are that small."""
+    import hbq_b200 as h
+    D = 64
+    g = torch.Generator(device="cuda").manual_seed(S + L)
+    r = lambda *s: torch.randn(s, device="cuda", generator=g)  # noqa: E731
+    u = lambda *s: ((torch.rand(s, device="cuda", generator=g) * 0.9 + 0.1) * size * r(*s).sign()).bfloat16()  # noqa: E731
+    q, k, v = r(B, L, H, D).bfloat16(), r(B, Hkv, S, D).bfloat16(), u(B, Hkv, S, D)
+    pk, pv = r(Hkv, P, D).bfloat16(), u(Hkv, P, D)
+    lengths = torch.full((B,), S, dtype=torch.int32, device="cuda")
+    got = (h.shared_prefix_attention(q, pk, pv, k, v, lengths=lengths) if P else h.window_attention(q, k, v, window=window, sinks=sinks, lengths=lengths))
+    see = _sees(L, S, S, window, sinks, P)
+    for b in range(min(B, 3)):
+        kk, vv = (torch.cat((a, t[b]), 1).double().repeat_interleave(H // Hkv, 0) for a, t in ((pk, k), (pv, v)))
+        s = (q[b].double().transpose(0, 1) @ kk.transpose(-1, -2) / math.sqrt(D)).masked_fill(~see, -math.inf)
+        w = torch.softmax(s, -1)
+        o, mass = (w @ vv).transpose(0, 1), (w @ vv.abs()).transpose(0, 1)
+        assert bool(((got[b].double() - o).abs() <= o.abs() * 2.0 ** -8 + mass * (2.0 ** -8 * 1.01 + 2.0 ** -12) + 2.0 ** -127).all())
