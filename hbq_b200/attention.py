@@ -103,7 +103,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     the keys up to p that are among the last ``window`` ones, itself included, or among the first ``sinks`` of the sequence;
     ``window=0``: all of them.  A row that sees nothing (p below 0), and a row behind its sequence's end (p >= ``lengths[b]``, the
     padding of a batch of prompts), is 0.  What the cache holds behind a sequence's end, or where a row's mask hides it, does
-    not matter, infinities and NaNs among it.  ``L = 1`` is a decode step.  ``scale`` defaults to ``1 / sqrt(D)``.  The result may be given as
+    not matter, infinities and NaNs among it; an infinity that a row sees reaches its result however small its weight.  Scores, softmax and
+    sums are held in 32 bits.  Where the tensor-core kernel takes the call (many rows) each weight is rounded to the tensors' type before
+    its product, and the result's error is 1.2 to 1.4 times that of its own rounding.  ``L = 1`` is a decode step.  ``scale`` defaults to ``1 / sqrt(D)``.  The result may be given as
     ``out``, of any strides with a dense last axis, which overlaps no input."""
     # (a count beyond any cache, held to 64 bits)
     return _run("window_attention", q, k, v, None, None, min(int(window), 2 ** 62), min(int(sinks), 2 ** 62), scale, lengths, starts, out)
@@ -117,7 +119,8 @@ def shared_prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     ``k_prefix`` and ``v_prefix`` ``[Hkv, P, D]`` are the keys and values of the shared beginning; ``q``, ``k``, ``v``, ``lengths`` and
     ``starts`` are those of ``window_attention`` for what each sequence has of its own, counted from the end of the prefix.  A row
     sees the whole prefix and its sequence's own keys up to its position; with no own key yet (p below 0) the prefix alone;
-    rows behind their sequence's end are 0."""
+    rows behind their sequence's end are 0.  Weights are held as ``window_attention``'s, those of the prefix in the tensors' type
+    but for calls of a few rows and keys."""
     if k_prefix is None or v_prefix is None:
         raise ValueError("shared_prefix_attention needs the prefix; window_attention is the operator without one")
     return _run("shared_prefix_attention", q, k, v, k_prefix, v_prefix, 0, 0, scale, lengths, starts, out)

@@ -108,8 +108,8 @@ __device__ __forceinline__ void unpack(uint4 r0, uint4 r1, bool apart, float2 (&
 // few a token's heads are spread over the warps of its blocks (blockIdx.y).
 //
 // Bytes in flight are what it needs: a warp's next heads are loaded before it works on the present ones, and its first ones
-// before the block's angles are known (16384 tokens of 32 heads of 128: 47 us, 5.7 TB/s; 32 + 8 heads with
-// the norm: 66 us, 5.1 TB/s).
+// before the block's angles are known (16384 tokens of 32 heads of 128: 48 us, 5.6 TB/s; 32 + 8 heads with
+// the norm: 68 us, 4.9 TB/s).
 template <class E, int LANES, bool NORM>
 __global__ void __launch_bounds__(WARPS * 32, 6) rotary_kernel(const __grid_constant__ RotaryArgs a)
 {
