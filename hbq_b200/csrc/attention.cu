@@ -133,7 +133,6 @@ int attention_run(const hbq_attention* call, void* workspace, int64_t workspace_
         const int rc = attention_rows_launch(a, p->dtype, stream);
         if (rc) return rc;
     }
-    a.P = p->P;
     return c.join() ? attention_join_launch(a, p->dtype, stream) : HBQ_OK;
 }
 

@@ -48,6 +48,10 @@ __device__ __forceinline__ float exp2_fast(float x)
     return y;
 }
 
+// What a sum is multiplied by when its maximum is exceeded, or when it is joined: never zero, since the sum may be an infinity that a row
+// sees.  The smallest number there is, 2^-149, adds below 2^-20 to others.
+__device__ __forceinline__ float factor_of(float x) { return fmaxf(exp2_fast(x), __uint_as_float(1u)); }
+
 // The second of a call's two attention kernels reads nothing that the first writes, and the first lets it start only behind its
 // own wait, when all before it is complete: it need not wait for the first, and fills the SMs that the first leaves.  It
 // waits at its end instead (its inputs come from L2, past what an SM's cache may hold of them from before), so that the kernel behind it, which joins both kernels' parts, finds both complete.
@@ -77,61 +81,6 @@ __device__ __forceinline__ float* slot_sum(const AttnArgs& a, int block, int whi
 __device__ __forceinline__ float2* slot_weight(const AttnArgs& a, int block, int which, int row)
 {
     return reinterpret_cast<float2*>(a.slots + (int64_t)a.blocks * 2 * 16 * a.D) + (block * 2 + which) * 16 + row;
-}
-
-// The infinities and NaNs that row (b, i) sees in the 8 * PIECES columns from d0 on, one bit a column.  A weight that 16 bits round
-// to zero, or the negative second part of a weight, makes a NaN of an infinity: whoever writes a row's output asks here about
-// results that are NaN, in which alone such a thing can show, and an infinity that is seen counts however small its weight.
-// Lane k of n looks at every n-th key, past the SM's own cache (begin_beside), until all columns of `want` are NaN for good.
-template <class E> struct Infinity16;
-template <> struct Infinity16<__half> { static constexpr uint32_t BITS = 0x7C00u; };
-template <> struct Infinity16<__nv_bfloat16> { static constexpr uint32_t BITS = 0x7F80u; };
-struct Specials {
-    uint32_t above, below;                                   // infinities; NaNs are in both
-    __device__ __forceinline__ float in_place_of(float y, int column) const
-    {
-        const bool p = (above >> column) & 1u, m = (below >> column) & 1u;
-        return p && m ? __int_as_float(0x7FFFFFFF) : p ? INFINITY : m ? -INFINITY : y;
-    }
-};
-template <class E, int PIECES>
-__device__ __noinline__ Specials specials_of(const AttnArgs& a, uint32_t b, uint32_t i, uint32_t hk, uint32_t d0, int k, int n, uint32_t want)
-{
-    constexpr uint32_t INF = Infinity16<E>::BITS;
-    Specials s = {0, 0};
-    int64_t len, p;
-    sequence_of(a, b, &len, &p);
-    p += i;
-    if (p >= len) return s;
-    #pragma unroll 1
-    for (int run = 0; run < 3; ++run) {            // the prefix, the first keys, those from lo on
-        const int64_t lo = p >= 0 && a.window > 0 && p >= a.window ? p - a.window + 1 : 0;
-        const int64_t first = run == 2 ? lo : 0, last = run == 0 ? a.P : run == 1 ? (a.sinks < lo ? a.sinks : lo) : p + 1;
-        const int64_t step = run == 0 ? a.pvs[1] : a.vs[2];
-        const uint16_t* v = (run == 0 ? static_cast<const uint16_t*>(a.pv) + (int64_t)hk * a.pvs[0]
-                                      : static_cast<const uint16_t*>(a.v) + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[1]) + d0 + (first + k) * step;
-        #pragma unroll 1
-        for (int64_t j = first + k; j < last && (s.above & s.below & want) != want; j += n, v += n * step) {
-            uint4 x[PIECES];
-            #pragma unroll
-            for (int c = 0; c < PIECES; ++c) x[c] = c == 0 || d0 + 8 * c < a.D ? __ldcg(reinterpret_cast<const uint4*>(v + 8 * c)) : make_uint4(0, 0, 0, 0);
-            #pragma unroll
-            for (int c = 0; c < PIECES; ++c) {
-                constexpr uint32_t EXPONENTS = INF * 0x10001u, ONE = (0x8000u - INF) * 0x10001u;
-                // (an exponent of ones and one more sets the bit above it)
-                if (!((((x[c].x & EXPONENTS) + ONE) | ((x[c].y & EXPONENTS) + ONE) | ((x[c].z & EXPONENTS) + ONE) | ((x[c].w & EXPONENTS) + ONE)) & 0x80008000u)) continue;
-                #pragma unroll 1
-                for (int e = 0; e < 8; ++e) {
-                    const uint32_t u = (e < 4 ? (e < 2 ? x[c].x : x[c].y) : e < 6 ? x[c].z : x[c].w) >> (16 * (e & 1)) & 0xFFFFu;
-                    if ((u & INF) != INF) continue;
-                    const bool nan = (u & 0x7FFFu) != INF;
-                    if (nan || u < 0x8000u) s.above |= 1u << (8 * c + e);
-                    if (nan || u >= 0x8000u) s.below |= 1u << (8 * c + e);
-                }
-            }
-        }
-    }
-    return s;
 }
 
 // attention_rows.cu

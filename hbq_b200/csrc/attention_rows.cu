@@ -22,6 +22,7 @@
 // block ends at 54.
 #include "attention_dev.cuh"
 #include "tc_dev.cuh"
+#include <type_traits>
 
 namespace hbq {
 
@@ -34,6 +35,7 @@ constexpr uint32_t POLLS = 1u << 20;
 
 template <class E> struct Mma;
 template <> struct Mma<__half> {
+    static constexpr uint32_t ONES = 0x3C003C00u, INF = 0x7C00u;
     static __device__ __forceinline__ void run(float* c, const uint32_t* a, uint32_t b0, uint32_t b1)
     {
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -44,6 +46,7 @@ template <> struct Mma<__half> {
     static __device__ __forceinline__ void store(void* p, int64_t i, float v) { static_cast<__half*>(p)[i] = __float2half_rn(v); }
 };
 template <> struct Mma<__nv_bfloat16> {
+    static constexpr uint32_t ONES = 0x3F803F80u, INF = 0x7F80u;
     static __device__ __forceinline__ void run(float* c, const uint32_t* a, uint32_t b0, uint32_t b1)
     {
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -150,8 +153,9 @@ __device__ void count_units(const AttnArgs& a, int64_t* table)
     __syncthreads();
 }
 
+// (240 registers, as the walk that keeps infinities apart would like more: with 255 the kernel behind it finds no room beside it, 98.9 -> 100.6 us)
 template <class E, int NK>
-__global__ void __launch_bounds__(RW * 32, BLOCKS_PER_SM) attention_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ RowsMaps maps, uint32_t tiles)
+__global__ void __maxnreg__(240) attention_rows_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ RowsMaps maps, uint32_t tiles)
 {
     using Sh = RowsShape<NK>;
     constexpr float SHIFT = Weights<E>::SHIFT;
@@ -227,13 +231,15 @@ __global__ void __launch_bounds__(RW * 32, BLOCKS_PER_SM) attention_rows_kernel(
         }
     };
     const int first = x0 + rank * RW + warp;
-    if (lane == 0 && ok) {
+    auto load_first = [&] {
+        if (lane != 0 || !ok) return;
         uint32_t st = stage;
         for (int k = 0; k < STAGES && first + k * stride < x1; ++k) {
             load(first + k * stride, st);
             if (++st == STAGES) st = 0;
         }
-    }
+    };
+    load_first();
 
     // queries as the left operand's fragments: rows lane / 4 and lane / 4 + 8
     uint32_t qf[NK][4];
@@ -245,96 +251,138 @@ __global__ void __launch_bounds__(RW * 32, BLOCKS_PER_SM) attention_rows_kernel(
             qf[kk][f] = r < rows && d < a.D
                 ? __ldcg(reinterpret_cast<const unsigned*>(static_cast<const E*>(a.q) + (int64_t)b * a.qs[0] + (int64_t)i * a.qs[1] + (int64_t)(h0 + r) * a.qs[2] + d)) : 0u;
         }
-    float o[NK * 2][4];
-    #pragma unroll
-    for (int t = 0; t < NK * 2; ++t)
-        #pragma unroll
-        for (int f = 0; f < 4; ++f) o[t][f] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    const float c = a.scale_log2;
 
-    for (int x = first; x < x1 && ok; x += stride) {
-        {
-            uint32_t it = 0;
-            while (!__all_sync(0xFFFFFFFFu, mbar_try_wait(bars + 8 * stage, phase)))
-                if (++it == POLLS) { ok = false; break; }
-            if (!ok) {
-                if (lane == 0) { *abort_flag = 1; atomicCAS(&g_tc_status, 0, 51); }
-                __syncwarp();
-                break;
-            }
-        }
-        const uint32_t kt = ring + stage * Sh::STAGE, vt = kt + Sh::TILE;
-        const int run = x < list.pre ? list.P - x * GROUP : x < list.sink ? list.ns - (x - list.pre) * GROUP : list.end - list.lo - (x - list.sink) * GROUP;
-        if (run < GROUP) {                                           // values behind the run's end
-            for (int y = lane; y < (GROUP - run) * Sh::HALVES * 8; y += 32) {
-                const int key = run + y / (Sh::HALVES * 8), pc = y % (Sh::HALVES * 8);
-                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vt + (pc >> 3) * (GROUP * 128) + key * 128 + (pc & 7) * 16), "r"(0) : "memory");
-            }
-            __syncwarp();
-        }
-        float s[2][4] = {};
+    float o[NK * 2][4], m[2], l[2];
+    const float c = a.scale_log2;
+    // The warp's steps.  A weight's second number may be zero or negative, and makes a NaN of an infinity among the values: `apart`
+    // takes infinities and NaNs out of the products and multiplies them by one.
+    const auto walk = [&](auto apart) {
+        constexpr bool APART = decltype(apart)::value;
         #pragma unroll
-        for (int kk = 0; kk < NK; ++kk) {
-            uint32_t f[4];
-            const int row = (lane & 7) + 8 * (lane >> 4), pc = (kk & 3) * 2 + ((lane >> 3) & 1);
-            ldsm4(f, kt + (kk >> 2) * (GROUP * 128) + row * 128 + ((pc ^ (row & 7)) * 16));
-            Mma<E>::run(s[0], qf[kk], f[0], f[1]);
-            Mma<E>::run(s[1], qf[kk], f[2], f[3]);
-        }
-        if (run < GROUP) {
+        for (int t = 0; t < NK * 2; ++t)
             #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if ((e >> 2) * 8 + (lane & 3) * 2 + (e & 1) >= run) s[e >> 2][e & 3] = -INFINITY;
-        }
-        float top[2];
-        #pragma unroll
-        for (int r = 0; r < 2; ++r) top[r] = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
-        if (__any_sync(0xFFFFFFFFu, (top[0] - m[0]) * c > GROWTH || (top[1] - m[1]) * c > GROWTH)) {
-            #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 1));
-                top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 2));
-                if (top[r] > m[r]) {
-                    const float f = exp2_fast((m[r] - top[r]) * c);
-                    m[r] = top[r];
-                    l[r] *= f;
-                    #pragma unroll
-                    for (int t = 0; t < NK * 2; ++t) { o[t][2 * r] *= f; o[t][2 * r + 1] *= f; }
+            for (int f = 0; f < 4; ++f) o[t][f] = 0.f;
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = 0.f;
+        for (int x = first; x < x1 && ok; x += stride) {
+            {
+                uint32_t it = 0;
+                while (!__all_sync(0xFFFFFFFFu, mbar_try_wait(bars + 8 * stage, phase)))
+                    if (++it == POLLS) { ok = false; break; }
+                if (!ok) {
+                    if (lane == 0) { *abort_flag = 1; atomicCAS(&g_tc_status, 0, 51); }
+                    __syncwarp();
+                    break;
                 }
             }
-        }
-        uint32_t hi[4], rest[4];
-        #pragma unroll
-        for (int r = 0; r < 2; ++r) {                                // row lane / 4 + 8 r
-            const float off = SHIFT - (m[r] == -INFINITY ? 0.f : m[r] * c);
-            #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float w0 = exp2_fast(fmaf(s[e][2 * r], c, off)), w1 = exp2_fast(fmaf(s[e][2 * r + 1], c, off));
-                l[r] += w0 + w1;
-                // the weights as two numbers of the values' type, so that their rounding does not reach the result (the second may
-                // be negative, and makes a NaN of an infinity among the values: specials_of)
-                hi[2 * e + r] = Mma<E>::pack(w0, w1);
-                const float2 back = Mma<E>::unpack(hi[2 * e + r]);
-                rest[2 * e + r] = Mma<E>::pack(w0 - back.x, w1 - back.y);
+            const uint32_t kt = ring + stage * Sh::STAGE, vt = kt + Sh::TILE;
+            const int run = x < list.pre ? list.P - x * GROUP : x < list.sink ? list.ns - (x - list.pre) * GROUP : list.end - list.lo - (x - list.sink) * GROUP;
+            if (run < GROUP) {                                           // values behind the run's end
+                for (int y = lane; y < (GROUP - run) * Sh::HALVES * 8; y += 32) {
+                    const int key = run + y / (Sh::HALVES * 8), pc = y % (Sh::HALVES * 8);
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vt + (pc >> 3) * (GROUP * 128) + key * 128 + (pc & 7) * 16), "r"(0) : "memory");
+                }
+                __syncwarp();
             }
+            float s[2][4] = {};
+            #pragma unroll
+            for (int kk = 0; kk < NK; ++kk) {
+                uint32_t f[4];
+                const int row = (lane & 7) + 8 * (lane >> 4), pc = (kk & 3) * 2 + ((lane >> 3) & 1);
+                ldsm4(f, kt + (kk >> 2) * (GROUP * 128) + row * 128 + ((pc ^ (row & 7)) * 16));
+                Mma<E>::run(s[0], qf[kk], f[0], f[1]);
+                Mma<E>::run(s[1], qf[kk], f[2], f[3]);
+            }
+            if (run < GROUP) {
+                #pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if ((e >> 2) * 8 + (lane & 3) * 2 + (e & 1) >= run) s[e >> 2][e & 3] = -INFINITY;
+            }
+            float top[2];
+            #pragma unroll
+            for (int r = 0; r < 2; ++r) top[r] = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
+            if (__any_sync(0xFFFFFFFFu, (top[0] - m[0]) * c > GROWTH || (top[1] - m[1]) * c > GROWTH)) {
+                #pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 1));
+                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 2));
+                    if (top[r] > m[r]) {
+                        const float f = factor_of((m[r] - top[r]) * c);
+                        m[r] = top[r];
+                        l[r] *= f;
+                        #pragma unroll
+                        for (int t = 0; t < NK * 2; ++t) { o[t][2 * r] *= f; o[t][2 * r + 1] *= f; }
+                    }
+                }
+            }
+            uint32_t hi[4], rest[4];
+            #pragma unroll
+            for (int r = 0; r < 2; ++r) {                                // row lane / 4 + 8 r
+                const float off = SHIFT - (m[r] == -INFINITY ? 0.f : m[r] * c);
+                #pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float w0 = exp2_fast(fmaf(s[e][2 * r], c, off)), w1 = exp2_fast(fmaf(s[e][2 * r + 1], c, off));
+                    l[r] += w0 + w1;
+                    // the weights as two numbers of the values' type, so that their rounding does not reach the result
+                    hi[2 * e + r] = Mma<E>::pack(w0, w1);
+                    const float2 back = Mma<E>::unpack(hi[2 * e + r]);
+                    rest[2 * e + r] = Mma<E>::pack(w0 - back.x, w1 - back.y);
+                }
+            }
+            if constexpr (!APART) {
+                #pragma unroll
+                for (int t = 0; t < NK; ++t) {
+                    uint32_t f[4];
+                    const int row = (lane & 7) + 8 * ((lane >> 3) & 1), pc = (t & 3) * 2 + (lane >> 4);
+                    ldsm4t(f, vt + (t >> 2) * (GROUP * 128) + row * 128 + ((pc ^ (row & 7)) * 16));
+                    Mma<E>::run(o[2 * t], hi, f[0], f[1]);
+                    Mma<E>::run(o[2 * t], rest, f[0], f[1]);
+                    Mma<E>::run(o[2 * t + 1], hi, f[2], f[3]);
+                    Mma<E>::run(o[2 * t + 1], rest, f[2], f[3]);
+                }
+            } else {
+                const uint32_t one[4] = {Mma<E>::ONES, Mma<E>::ONES, Mma<E>::ONES, Mma<E>::ONES};
+                #pragma unroll
+                for (int t = 0; t < NK; ++t) {
+                    uint32_t f[4], g[4];
+                    const int row = (lane & 7) + 8 * ((lane >> 3) & 1), pc = (t & 3) * 2 + (lane >> 4);
+                    ldsm4t(f, vt + (t >> 2) * (GROUP * 128) + row * 128 + ((pc ^ (row & 7)) * 16));
+                    #pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        constexpr uint32_t INF = Mma<E>::INF;
+                        g[e] = f[e] & (((f[e] & INF) == INF ? 0x0000FFFFu : 0u) | ((f[e] & (INF << 16)) == INF << 16 ? 0xFFFF0000u : 0u));
+                        f[e] ^= g[e];
+                    }
+                    #pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        Mma<E>::run(o[2 * t + e], hi, f[2 * e], f[2 * e + 1]);
+                        Mma<E>::run(o[2 * t + e], rest, f[2 * e], f[2 * e + 1]);
+                        Mma<E>::run(o[2 * t + e], one, g[2 * e], g[2 * e + 1]);
+                    }
+                }
+            }
+            __syncwarp();                                                // every lane has read the stage
+            if (lane == 0 && x + STAGES * stride < x1) {
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                load(x + STAGES * stride, stage);
+            }
+            if (++stage == STAGES) { stage = 0; phase ^= 1u; }
         }
+    };
+    walk(std::false_type());
+    {
+        float nan[4] = {o[0][0], o[0][1], o[0][2], o[0][3]};
         #pragma unroll
-        for (int t = 0; t < NK; ++t) {
-            uint32_t f[4];
-            const int row = (lane & 7) + 8 * ((lane >> 3) & 1), pc = (t & 3) * 2 + (lane >> 4);
-            ldsm4t(f, vt + (t >> 2) * (GROUP * 128) + row * 128 + ((pc ^ (row & 7)) * 16));
-            Mma<E>::run(o[2 * t], hi, f[0], f[1]);
-            Mma<E>::run(o[2 * t], rest, f[0], f[1]);
-            Mma<E>::run(o[2 * t + 1], hi, f[2], f[3]);
-            Mma<E>::run(o[2 * t + 1], rest, f[2], f[3]);
+        for (int t = 1; t < NK * 2; ++t)
+            #pragma unroll
+            for (int f = 0; f < 4; f += 2) asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(nan[(t & 1) * 2 + f / 2]) : "f"(o[t][f]), "f"(o[t][f + 1]));
+        asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(nan[0]) : "f"(nan[1]), "f"(nan[2]));
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(nan[0]) : "f"(nan[3]));
+        if (__builtin_expect(__any_sync(0xFFFFFFFFu, nan[0] != nan[0]) && ok, 0)) {             // once more: twice the time of a group that holds one
+            if (lane == 0) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            load_first();
+            walk(std::true_type());
         }
-        __syncwarp();                                                // every lane has read the stage
-        if (lane == 0 && x + STAGES * stride < x1) {
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            load(x + STAGES * stride, stage);
-        }
-        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
     }
     #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -349,9 +397,7 @@ __global__ void __launch_bounds__(RW * 32, BLOCKS_PER_SM) attention_rows_kernel(
             part_sum(a, at, a.part0)[d] = sum;
             if (d == 0) *part_weight(a, at, a.part0) = make_float2(top, weight);
         } else {
-            float y = weight == 0.f ? 0.f : sum / weight;
-            if (y != y && weight == weight) y = specials_of<E, 1>(a, b, i, hk, d & ~7u, 0, 1, 1u << (d & 7)).in_place_of(y, d & 7);
-            Mma<E>::store(a.out, (int64_t)b * a.os[0] + (int64_t)i * a.os[1] + (int64_t)(h0 + row) * a.os[2] + d, y);
+            Mma<E>::store(a.out, (int64_t)b * a.os[0] + (int64_t)i * a.os[1] + (int64_t)(h0 + row) * a.os[2] + d, weight == 0.f ? 0.f : sum / weight);
         }
     };
     float* block = reinterpret_cast<float*>(smem + Sh::JOIN);
@@ -381,7 +427,7 @@ __global__ void __launch_bounds__(RW * 32, BLOCKS_PER_SM) attention_rows_kernel(
         const float ref = top == -INFINITY ? 0.f : top;
         #pragma unroll
         for (int w = 0; w < RW; ++w) {
-            const float f = exp2_fast(jm[(w * 16 + row) * 2] - ref);
+            const float f = factor_of(jm[(w * 16 + row) * 2] - ref);
             sum = fmaf(js[(w * 16 + row) * Sh::DP + d], f, sum);
             weight = fmaf(jm[(w * 16 + row) * 2 + 1], f, weight);
         }
@@ -410,7 +456,7 @@ __global__ void __launch_bounds__(RW * 32, BLOCKS_PER_SM) attention_rows_kernel(
             #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 if (weights[k] == 0.f) continue;                     // (a NaN is no zero)
-                const float f = exp2_fast(tops[k] - ref);
+                const float f = factor_of(tops[k] - ref);
                 sum = fmaf(sums[k], f, sum);
                 weight = fmaf(weights[k], f, weight);
             }
@@ -439,7 +485,7 @@ __global__ void __launch_bounds__(RW * 32, BLOCKS_PER_SM) attention_rows_kernel(
 // sums relative to the largest.  A chain of dependent loads, bound by their latency: the blocks of a group come from its
 // table entry, and with few rows four warps share a row's parts (8 rows of 37 parts: 8.4 -> 5 us).
 template <class E, int W>
-__global__ void __launch_bounds__(128, W > 1 ? 16 : 12) attention_join_kernel(const __grid_constant__ AttnArgs a, uint32_t tiles)
+__global__ void __launch_bounds__(128) attention_join_kernel(const __grid_constant__ AttnArgs a, uint32_t tiles)
 {
     __shared__ float sums[W > 1 ? W : 1][128], weights[W > 1 ? W : 1];
     grid_dependency_wait();
@@ -475,8 +521,7 @@ __global__ void __launch_bounds__(128, W > 1 ? 16 : 12) attention_join_kernel(co
         float f = 0.f;
         if (s0 + lane * W < count) {
             const float2 ml = weight_of(s0 + lane * W);
-            // (no part that saw a key counts for nothing: its sum may be an infinity.  The smallest number there is, 2^-149, adds below 2^-20)
-            if (ml.y != 0.f) { f = fmaxf(exp2_fast(ml.x - ref), __uint_as_float(1u)); weight = fmaf(ml.y, f, weight); }
+            if (ml.y != 0.f) { f = factor_of(ml.x - ref); weight = fmaf(ml.y, f, weight); }
         }
         const int end = min(32, (count - s0 + W - 1) / W);
         #pragma unroll 8
@@ -504,25 +549,10 @@ __global__ void __launch_bounds__(128, W > 1 ? 16 : 12) attention_join_kernel(co
         }
     }
     const uint32_t b = token / a.L, i = token - b * a.L;
-    const int64_t at = (int64_t)b * a.os[0] + (int64_t)i * a.os[1] + (int64_t)h * a.os[2];
-    bool odd = false;
     if (in) {
         #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float y = weight == 0.f ? 0.f : sum[e] / weight;
-            odd |= y != y;
-            Mma<E>::store(a.out, at + lane * 4 + e, y);
-        }
-    }
-    uint32_t lanes = __ballot_sync(0xFFFFFFFFu, odd && weight == weight);
-    while (lanes) {                                                  // eight columns with a NaN among them: two lanes'
-        const int piece = (__ffs(lanes) - 1) / 2;
-        lanes &= ~(3u << (2 * piece));
-        Specials s = specials_of<E, 1>(a, b, i, h / a.G, piece * 8, lane, 32, 0xFFu);
-        s.above = __reduce_or_sync(0xFFFFFFFFu, s.above);
-        s.below = __reduce_or_sync(0xFFFFFFFFu, s.below);
-        __syncwarp();                                                // (behind the stores of the same values above)
-        if (lane < 8 && ((s.above | s.below) >> lane & 1u)) Mma<E>::store(a.out, at + piece * 8 + lane, s.in_place_of(0.f, lane));
+        for (int e = 0; e < 4; ++e)
+            Mma<E>::store(a.out, (int64_t)b * a.os[0] + (int64_t)i * a.os[1] + (int64_t)h * a.os[2] + lane * 4 + e, weight == 0.f ? 0.f : sum[e] / weight);
     }
 }
 

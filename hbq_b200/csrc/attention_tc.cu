@@ -11,8 +11,8 @@
 // Keys come by TMA in a ring that keys and values share, from a cache of any strides.  Tiles that the masks of all rows hide
 // are left out; the mask is applied only in tiles that hide some key from some row.  There the weights hold zeros, and a
 // zero times an infinity or a NaN of a hidden value would still reach the sum: such values are set to zero in shared memory
-// before the product, and the rows that do see them get them added at the end.  An infinity of a tile that all rows see
-// becomes a NaN where a row's weight rounds to zero: a result that is NaN is looked into (specials_of).
+// before the product, and the rows of such a block are given what they see of them at the end (give_specials).  An infinity of a tile
+// that all rows see becomes a NaN where a row's weight rounds to zero: a row that ends with a NaN is looked into likewise.
 //
 // What bounds it: per pair of 128 x 128 tiles the products take 2048 cycles at heads of 128, and shared memory delivers their operands in
 // as many; the powers of two take 2048 on the special-function unit, a quarter of which is computed on the FMA pipe instead.  A
@@ -180,6 +180,78 @@ struct Span {
     }
     __device__ __forceinline__ bool seen_by_some(int j) const { return j <= pb && (window == 0 || j > pa - window || j < sinks); }
 };
+
+// Puts the infinities and NaNs that row (b, i) of each `wanted` lane sees, of the prefix or of its own keys, into 32 columns (from d0 on) of
+// its sums in tensor memory.  By a whole warp, out of line, past the SM's own cache (begin_beside).  The keys that all wanted
+// rows see are shared out among the lanes, the rest of a row's are its lane's (a lane for all of its row's: 56 ms for 8192
+// tokens in place of 4).  Of all keys for a piece of them too: the pieces' sum is what it is in each.
+template <class E>
+__device__ __noinline__ void give_specials(const AttnArgs& a, int prefix, uint32_t b, uint32_t i, uint32_t hk, int d0, bool wanted, uint32_t sums)
+{
+    constexpr uint32_t INF = Word<E>::INF, EXPONENTS = INF * 0x10001u, ONE = (0x8000u - INF) * 0x10001u;
+    const uint16_t* v = (prefix ? static_cast<const uint16_t*>(a.pv) + (int64_t)hk * a.pvs[0]
+                                : static_cast<const uint16_t*>(a.v) + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[1]) + d0;
+    const int64_t step = prefix ? a.pvs[1] : a.vs[2];
+    int lo = 0, end = 0, first = 0;                          // this row's keys: those before `first`, and lo .. end - 1
+    if (wanted) {
+        int64_t n, p;
+        sequence_of(a, b, &n, &p);
+        p += i;
+        lo = !prefix && a.window > 0 && p >= a.window ? (int)(p - a.window + 1) : 0;
+        end = prefix ? (int)a.P : (int)p + 1;
+        first = a.sinks < lo ? (int)a.sinks : lo;
+    }
+    int all_lo = __reduce_max_sync(0xFFFFFFFFu, lo), all_end = __reduce_min_sync(0xFFFFFFFFu, wanted ? end : 0x7FFFFFFF);
+    const int all_first = __reduce_min_sync(0xFFFFFFFFu, wanted ? first : 0x7FFFFFFF);
+    if (all_lo >= all_end) all_lo = all_end = 0x7FFFFFFF;    // nothing in common
+    const int lane = threadIdx.x & 31;
+    uint32_t above = 0, below = 0;                           // a bit a column: infinities; NaNs are in both
+    #pragma unroll 1
+    for (int run = 0; run < 5; ++run) {
+        if (run == 2) {
+            above = __reduce_or_sync(0xFFFFFFFFu, above);
+            below = __reduce_or_sync(0xFFFFFFFFu, below);
+        }
+        const int n = run < 2 ? 32 : 1;
+        const int j0 = run == 0 ? lane : run == 1 ? (all_lo < all_end ? all_lo + lane : 0) : run == 2 ? all_first : run == 3 ? lo : max(all_end, lo);
+        const int j1 = run == 0 ? all_first : run == 1 ? (all_lo < all_end ? all_end : 0) : run == 2 ? first : run == 3 ? min(all_lo, end) : end;
+        #pragma unroll 1
+        for (int64_t j = j0; j < j1 && (above & below) != 0xFFFFFFFFu; j += 2 * n) {
+            uint4 x[8];                                      // two keys' four pieces of eight columns
+            #pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                const int64_t key = j + (c >> 2) * n;
+                x[c] = make_uint4(0, 0, 0, 0);
+                if (key < j1 && d0 + 8 * (c & 3) < (int)a.D) x[c] = __ldcg(reinterpret_cast<const uint4*>(v + key * step + 8 * (c & 3)));
+            }
+            #pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                // (an exponent of ones and one more sets the bit above it)
+                if (!((((x[c].x & EXPONENTS) + ONE) | ((x[c].y & EXPONENTS) + ONE) | ((x[c].z & EXPONENTS) + ONE) | ((x[c].w & EXPONENTS) + ONE)) & 0x80008000u)) continue;
+                #pragma unroll 1
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t u = (e < 4 ? (e < 2 ? x[c].x : x[c].y) : e < 6 ? x[c].z : x[c].w) >> (16 * (e & 1)) & 0xFFFFu, bit = 1u << (8 * (c & 3) + e);
+                    if ((u & INF) != INF) continue;
+                    const bool is_nan = (u & 0x7FFFu) != INF;
+                    if (is_nan || u < 0x8000u) above |= bit;
+                    if (is_nan || u >= 0x8000u) below |= bit;
+                }
+            }
+        }
+        __syncwarp();
+    }
+    float o[32];
+    tc_ld32(sums, o);
+    uint32_t w[32];
+    #pragma unroll
+    for (int e = 0; e < 32; ++e) {
+        const bool p = wanted && ((above >> e) & 1u), m = wanted && ((below >> e) & 1u);
+        w[e] = p && m ? 0x7FFFFFFFu : p ? 0x7F800000u : m ? 0xFF800000u : __float_as_uint(o[e]);
+    }
+    tc_st16(sums, w);
+    tc_st16(sums + 16, w + 16);
+    tc_st_wait();
+}
 
 template <class E, int DP>
 __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -437,7 +509,7 @@ __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_const
             const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
             const bool grow = (top - m) * c > GROWTH;        // (from -inf: any; -inf itself: NaN, false)
             if (__any_sync(0xFFFFFFFFu, grow)) {
-                const float f = grow ? exp2_fast((m - top) * c) : 1.f;
+                const float f = grow ? factor_of((m - top) * c) : 1.f;
                 if (grow) m = top;
                 l *= f;
                 if (u > 0) {
@@ -506,45 +578,22 @@ __global__ void __launch_bounds__(TCT, 1) attention_tc_kernel(const __grid_const
                     float o[32];
                     __syncwarp();
                     if (nt > 0) tc_ld32(o_col + 32 * k, o);
+                    // (chains of maxima find a NaN with half the instructions of 32 comparisons: short prompts 29.6 -> 28.7 us)
+                    float nan[4] = {o[28], o[29], o[30], o[31]};
+                    #pragma unroll
+                    for (int e = 0; e < 28; e += 2) asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(nan[(e >> 1) & 3]) : "f"(o[e]), "f"(o[e + 1]));
+                    asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(nan[0]) : "f"(nan[1]), "f"(nan[2]));
+                    asm("max.NaN.f32 %0, %0, %1;" : "+f"(nan[0]) : "f"(nan[3]));
+                    const bool look = live && l == l && (add || nan[0] != nan[0]);
+                    if (__builtin_expect(__any_sync(0xFFFFFFFFu, look), 0)) {
+                        give_specials<E>(a, task.prefix, b, i, hk, 32 * k, look, o_col + 32 * k);
+                        tc_ld32(o_col + 32 * k, o);
+                    }
                     if (!live) {
                         #pragma unroll
                         for (int e = 0; e < 32; ++e) o[e] = 0.f;
                     }
-                    if (add && live) {
-                        const E* v = task.prefix ? static_cast<const E*>(a.pv) + (int64_t)hk * a.pvs[0]
-                                                 : static_cast<const E*>(a.v) + (int64_t)group * a.vs[0] + (int64_t)hk * a.vs[1];
-                        const int64_t vstep = task.prefix ? a.pvs[1] : a.vs[2];
-                        for (int u = u0; u < u1; ++u) {
-                            const int j0 = sp.tile(u) * TILE;
-                            if (sp.whole(j0)) continue;
-                            for (int j = j0; j < j0 + TILE && j <= hi; ++j) {
-                                if (j < lo && j >= sp.sinks) continue;
-                                #pragma unroll 1
-                                for (int e = 0; e < 32; ++e) {
-                                    if (32 * k + e >= (int)a.D) break;
-                                    const float x = Word<E>::up(__ldcg(reinterpret_cast<const uint16_t*>(v) + j * vstep + 32 * k + e));     // (begin_beside)
-                                    if (!isfinite(x)) {
-                                        #pragma unroll
-                                        for (int z = 0; z < 32; ++z) if (z == e) o[z] += x;
-                                    }
-                                }
-                            }
-                        }
-                    }
                     if (direct) {
-                        // (a chain of maxima finds a NaN with half the instructions of 32 comparisons: short prompts 29.6 -> 28.7 us)
-                        float nan[2] = {o[30], o[31]};
-                        #pragma unroll
-                        for (int e = 0; e < 30; e += 2) asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(nan[(e >> 1) & 1]) : "f"(o[e]), "f"(o[e + 1]));
-                        asm("max.NaN.f32 %0, %0, %1;" : "+f"(nan[0]) : "f"(nan[1]));
-                        if (nan[0] != nan[0] && l == l) {
-                            uint32_t odd = 0;
-                            #pragma unroll
-                            for (int e = 0; e < 32; ++e) if (o[e] != o[e]) odd |= 1u << e;
-                            const Specials s = specials_of<E, 4>(a, b, i, hk, 32 * k, 0, 1, odd);
-                            #pragma unroll
-                            for (int e = 0; e < 32; ++e) if (o[e] != o[e]) o[e] = s.in_place_of(o[e], e);
-                        }
                         uint32_t w[16];
                         #pragma unroll
                         for (int z = 0; z < 16; ++z) w[z] = Word<E>::pack(o[2 * z] * f, o[2 * z + 1] * f);

@@ -129,3 +129,27 @@ def test_values_at_the_ends_of_bf16(B, L, H, Hkv, S, P, window, sinks, size):
         w = torch.softmax(s, -1)
         o, mass = (w @ vv).transpose(0, 1), (w @ vv.abs()).transpose(0, 1)
         assert bool(((got[b].double() - o).abs() <= o.abs() * 2.0 ** -8 + mass * (2.0 ** -8 * 1.01 + 2.0 ** -12) + 2.0 ** -127).all())
+
+
+@pytest.mark.parametrize("value", [INF, NAN])
+@pytest.mark.parametrize("B,L,S", [(1, 1, 131072), (300, 1, 4096), (1, 4096, 4096)])
+def test_a_special_value_does_not_stop_the_batch(B, L, S, value):
+    """One key's values of each head: the rows that see them take their keys once or twice more, not a lane's time for each key (which was
+    some hundred times the call)."""
+    import hbq_b200 as h
+    g = torch.Generator(device="cuda").manual_seed(5)
+    q = (torch.randn((B, L, 32, 128), device="cuda", generator=g) * 20).half()
+    k, v = (torch.randn((B, 8, S, 128), device="cuda", generator=g).half() for _ in range(2))
+
+    def time_of(n=5):
+        h.window_attention(q, k, v)
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        for _ in range(n):
+            h.window_attention(q, k, v)
+        b.record()
+        torch.cuda.synchronize()
+        return a.elapsed_time(b)
+    clean = time_of()
+    v[:, :, S // 3] = value
+    assert time_of() < 40 * clean
