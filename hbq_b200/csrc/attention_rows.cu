@@ -597,8 +597,8 @@ int rows_type(const AttnArgs& a, const RowsMaps& maps, cudaStream_t stream)
 // all are resident at once and none has more than 512 keys (8 steps a warp); else shares of equal size over the blocks that are
 // resident, or a block a group where there are too many tokens for the table.  us, 32 / 8 heads of 128, clusters and shares:
 // one sequence of 512 keys 8.9 and 9.2, 4096 12.2 and 16.7, 8192 18 and 19, 16384 30 and 22; 8 of 2048 14.9 and 22; 64 of 512
-// (a block each) 31 and 37.  256 sequences in shares and 257 in blocks: 1024 keys each 170 and 172, 16 to 1024 of them 131 and 105, one of
-// 32768 among 512s 115 and 411.  `*small`: all row groups are resident and have no more keys than that.
+// (a block each) 31 and 37.  256 sequences in shares and 257 in blocks: 1024 keys each 169 and 177, 16 to 1024 of them 130 and 106, one of
+// 32768 among 512s 117 and 427.  `*small`: all row groups are resident and have no more keys than that.
 int attention_rows_blocks(const hbq_attention* p, bool prefix, int* shared, int* cluster, bool* small)
 {
     int sms = 148;

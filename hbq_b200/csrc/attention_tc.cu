@@ -17,9 +17,9 @@
 // What bounds it: per pair of 128 x 128 tiles the products take 2048 cycles at heads of 128, and shared memory delivers their operands in
 // as many; the powers of two take 2048 on the special-function unit, a quarter of which is computed on the FMA pipe instead.  A
 // row tile's softmax (some 1700 cycles) and the products it waits for (1024 and 300 of hand-over) follow one another, since the weights
-// lie on the scores: tensor memory has no room for both.  The tensor pipe is busy 52 to 54 % of the time.  8192 tokens, 32 / 8 heads of
+// lie on the scores: tensor memory has no room for both.  The tensor pipe is busy 51 to 53 % of the time.  8192 tokens, 32 / 8 heads of
 // 128, bf16, 20 calls in a row: all keys 459 us, 1197 TFLOP/s; window of 4096 374 us, 1103 of visible pairs; under a sustained
-// load, where the power cap holds the clock at 1.67 GHz, 442 us.  A block of one key tile takes some 7 us.
+// load, where the power cap holds the clock at 1.65 to 1.67 GHz, 442 to 453 us.  A block of one key tile takes some 7 us.
 #include "attention_dev.cuh"
 #include "tc_dev.cuh"
 
