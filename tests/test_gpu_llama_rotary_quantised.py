@@ -125,3 +125,27 @@ def test_prefill_in_runs_holds_no_square_of_scores(kind):
     at(x, B, T, cos, sin)
     # queries, keys, values, outputs and their copies are below 16 of [T, 4, 128]; the square of scores alone is four heads of T * T
     assert torch.cuda.max_memory_allocated() - before < 16 * T * 4 * 128 * 2 + 4 * T * 256 * 2 * 2
+
+
+@torch.no_grad()
+def test_heads_beyond_the_one_pass_kernel_in_runs():
+    """Heads of 256 without quantizers take the masked path: runs against the whole prompt, and against the formula in fp64 of fp16
+    queries, keys and values.  Scores, probabilities and the output are each rounded to fp16: the scores' half step, 2^-11 of up to 8,
+    is at most 2^-8 of a weight; in a mean of many that is independent of the values, well below 2^-7 of its norm."""
+    import hbq_b200 as H
+    from hbq_b200.llama import QLlamaAttention
+    at = QLlamaAttention(H.LlamaArch(hidden=256, layers=1, heads=4, kv_heads=2, head_dim=256, ffn=512, vocab=512, window=100, sinks=5), device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(4)
+    B, T, D = 2, 512, 256
+    Q, K, V = (torch.randn((B, n, T, D), device="cuda", generator=g).half() for n in (4, 2, 2))
+    out = []
+    for chunk in (1 << 30, 128, 256):
+        at.query_chunk = chunk
+        out.append(at._windowed(Q, K, V).double())
+    i, j = torch.arange(T, device="cuda")[:, None], torch.arange(T, device="cuda")[None]
+    hidden = (j > i) | ((j <= i - 100) & (j >= 5))
+    s = (Q.double() @ K.double().repeat_interleave(2, 1).transpose(-1, -2) / 16).masked_fill(hidden, -math.inf)
+    want = (torch.softmax(s, -1) @ V.double().repeat_interleave(2, 1)).transpose(1, 2).reshape(B * T, -1)
+    for o in out:
+        assert float((o - out[0]).norm() / want.norm()) <= 2.0 ** -9
+        assert float((o - want).norm() / want.norm()) <= 2.0 ** -7
